@@ -24,6 +24,9 @@ LIB_PATH = _HERE / "libgraphzero_b200.so"
 TICTACTOE, CONNECT4, CHESS = 0, 1, 2
 GAT, RESNET = 0, 1
 PREC_AUTO, PREC_FP32, PREC_BF16, PREC_FP16 = 0, 1, 2, 3
+F32, F16, BF16 = 0, 1, 2
+POLICY_MAX_ACTIONS = 262144
+ADAMW_BLOCK = 256
 GAME_NAMES = {"tictactoe": TICTACTOE, "connect4": CONNECT4, "chess": CHESS}
 
 OK, ERR_INVALID_ARG, ERR_CUDA, ERR_NCCL, ERR_TIMEOUT, ERR_IO, ERR_CAPACITY, ERR_UNSUPPORTED = range(8)
@@ -61,6 +64,27 @@ class TrainConfig(C.Structure):
 
 class TrainStats(C.Structure):
     _fields_ = [("policy_loss", C.c_float), ("value_loss", C.c_float), ("steps", C.c_int64)]
+
+
+class PolicyRows(C.Structure):
+    """gz_policy_rows: rows of action scores and the legal moves."""
+    _fields_ = [("logits", _vp), ("mask", _vp), ("logits_stride", C.c_int64), ("mask_stride", C.c_int64),
+                ("rows", C.c_int64), ("actions", C.c_int32), ("dtype", C.c_int32)]
+
+
+class SampleConfig(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_int32),
+                ("d_temperature", _vp), ("d_top_p", _vp), ("d_min_p", _vp), ("d_top_k", _vp)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", _vp), ("copy", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp), ("v_scale", _vp),
+                ("n", C.c_int64), ("weight_decay", C.c_double), ("lr_scale", C.c_double), ("copy_dtype", C.c_int32)]
+
+
+class AdamWConfig(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("max_norm", C.c_double), ("grad_scale", C.c_float), ("step", C.c_int64), ("seed", C.c_uint64)]
 
 
 # name -> (restype, argtypes)
@@ -138,6 +162,12 @@ _SIGS = {
     "gz_train_batch_indices": (C.c_int, [C.c_int64, C.POINTER(TrainConfig), C.c_int, C.c_int64, C.c_int, C.c_int,
                                          C.POINTER(C.c_int64)]),
     "gz_train_bucket_range": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    "gz_policy_sample": (C.c_int, [C.POINTER(PolicyRows), C.POINTER(SampleConfig), _vp, C.c_int64, _vp, _vp, _vp]),
+    "gz_policy_loss": (C.c_int, [C.POINTER(PolicyRows), _vp, C.c_int64, _vp, _vp, C.c_float, _vp, _vp, C.c_int64,
+                                 _vp]),
+    "gz_adamw_create": (C.c_int, [C.POINTER(AdamWTensor), C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
+    "gz_adamw_destroy": (C.c_int, [_vp]),
+    "gz_adamw_step": (C.c_int, [_vp, C.POINTER(_vp), _i32p, C.POINTER(AdamWConfig), _vp, _vp]),
     "gz_gat_c4_predict_noalloc": (C.c_int, [C.c_int, _f32p, C.c_size_t, _i8p, _i8p, C.c_int, _f32p, _f32p]),
     "gz_gat_c4_noalloc_scratch_bytes": (C.c_size_t, []),
     "gz_gat_c4_noalloc_max_batch": (C.c_int, []),
@@ -660,6 +690,215 @@ def load_train_examples(path) -> list:
                                        n_it.value, C.byref(n_it), C.byref(total)))
     offs = np.concatenate([[0], np.cumsum(counts[:n_it.value])])
     return [out[offs[i]:offs[i + 1]] for i in range(n_it.value)]
+
+
+# ---- policies of the caller's own: drawing actions, loss, optimiser (gz_policy_*, gz_adamw_*) ----
+
+
+def _policy_rows(logits, mask):
+    """gz_policy_rows of torch tensors [rows][actions] (and what it points to)."""
+    import torch
+    dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if logits.dim() != 2 or logits.dtype not in dtypes or not logits.is_cuda:
+        raise ValueError("logits must be a [rows][actions] CUDA tensor of float32, float16 or bfloat16")
+    n, a = logits.shape
+    if a > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if mask is not None:
+        if mask.shape != logits.shape or mask.dtype not in (torch.uint8, torch.bool) or mask.device != logits.device:
+            raise ValueError("mask must be a uint8 or bool tensor of the logits' shape and device")
+        if a > 1 and mask.stride(1) != 1:
+            mask = mask.contiguous()
+    return logits, mask, PolicyRows(logits.data_ptr(), None if mask is None else mask.data_ptr(), logits.stride(0),
+                                    0 if mask is None else mask.stride(0), n, a, dtypes[logits.dtype])
+
+
+def _row_values(x, name, dtype, n, device):
+    """A [rows] tensor of the given type, contiguous."""
+    if x.shape != (n,) or x.dtype != dtype or x.device != device:
+        raise ValueError(f"{name} must be a [rows] tensor of {dtype} on the logits' device")
+    return x.contiguous()
+
+
+def _action_values(x, name, shape, device):
+    """A float32 [rows][actions] tensor whose rows are contiguous."""
+    import torch
+    if x.shape != shape or x.dtype != torch.float32 or x.device != device:
+        raise ValueError(f"{name} must be a float32 tensor of the logits' shape and device")
+    return x if shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+class _On:
+    """The tensor's device for the scope, entered only where it is not the current one."""
+
+    def __init__(self, device):
+        import torch
+        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=None):
+    """One action per row of `logits` (torch, [rows][actions], float32, float16
+    or bfloat16), drawn with `noise` (float32 standard Gumbel numbers of the
+    same shape, e.g. -torch.empty(...).exponential_().log(); None picks the
+    best action) among the actions that `mask` leaves visible and that
+    temperature, top_k, top_p and min_p keep.  Each setting is a number or a
+    [rows] tensor (float32; top_k int32).  Returns (action int32 [rows], -1
+    where nothing is visible; logp float32 [rows], the action's
+    log-probability among the kept ones).  See gz_policy_sample."""
+    import torch
+    logits, mask, rows = _policy_rows(logits, mask)
+    n, dev, cfg = logits.shape[0], logits.device, SampleConfig(1.0, 1.0, 0.0, 0)
+    kept = []  # what the settings point to
+    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(x, torch.Tensor):
+            kept.append(_row_values(x, name, dtype, n, dev))
+            setattr(cfg, "d_" + name, kept[-1].data_ptr())
+        else:
+            setattr(cfg, name, x)
+    if noise is not None:
+        noise = _action_values(noise, "noise", logits.shape, dev)
+    action = torch.empty(n, dtype=torch.int32, device=dev)
+    logp = torch.empty(n, dtype=torch.float32, device=dev)
+    with _On(dev):
+        _check(_lib.gz_policy_sample(C.byref(rows), C.byref(cfg), _dev(noise), 0 if noise is None else noise.stride(0),
+                                     action.data_ptr(), logp.data_ptr(), _stream(stream)))
+    return action, logp
+
+
+def policy_loss(logits, target=None, label=None, mask=None, weight=None, grad_scale=1.0, need_grad=True, stream=None):
+    """Cross-entropy of softmax(logits) over the actions that `mask` leaves
+    visible, and its gradient, in one pass: (loss float32 [rows], grad of the
+    logits' shape and type, or None without need_grad).  The targets are
+    `target` (float32 [rows][actions] amounts) or `label` (int32 [rows]);
+    `weight` (float32 [rows]) multiplies a row, `grad_scale` the gradient
+    alone (1 / rows for the mean loss).  Continue a torch backward pass with
+    logits.backward(grad).  See gz_policy_loss."""
+    import torch
+    logits, mask, rows = _policy_rows(logits, mask)
+    (n, a), dev = logits.shape, logits.device
+    if (target is None) == (label is None):
+        raise ValueError("give either target or label")
+    if target is not None:
+        target = _action_values(target, "target", logits.shape, dev)
+    else:
+        label = _row_values(label, "label", torch.int32, n, dev)
+    if weight is not None:
+        weight = _row_values(weight, "weight", torch.float32, n, dev)
+    loss = torch.empty(n, dtype=torch.float32, device=dev)
+    grad = torch.empty((n, a), dtype=logits.dtype, device=dev) if need_grad else None
+    with _On(dev):
+        _check(_lib.gz_policy_loss(C.byref(rows), _dev(target), 0 if target is None else target.stride(0), _dev(label),
+                                   _dev(weight), grad_scale, loss.data_ptr(), _dev(grad), a, _stream(stream)))
+    return loss, grad
+
+
+class AdamW:
+    """AdamW over a list of float32 CUDA tensors in one launch (gz_adamw_*).
+
+    `copies` are 16-bit tensors of the same shapes that every step writes the
+    new weights to (None where a weight has none); `copies`, `weight_decay` and
+    `lr_scale` are one value or one per tensor.  With max_norm > 0 the
+    gradients are scaled down to that global norm.  The states are flat tensors
+    over all weights, each tensor's share rounded up to whole blocks of
+    ADAMW_BLOCK and starting at offsets[k]: m and v (32 bits), or m and the
+    root of v as float8_e4m3fn with m_scale and v_scale per block (8 bits).
+    Together with `steps`, the number of steps taken, they are all there is to
+    save.  `lr` and `max_norm` may be changed between steps."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, copies=None,
+                 lr_scale=1.0, max_norm=0.0, seed=0):
+        import torch
+        self._plan = _vp()
+        self.params = list(params)
+        count = len(self.params)
+        each = lambda x: list(x) if isinstance(x, (list, tuple)) else [x] * count  # noqa: E731
+        self.copies, decays, scales = each(copies), each(weight_decay), each(lr_scale)
+        if not self.params:
+            raise ValueError("no tensors")
+        if any(len(x) != count for x in (self.copies, decays, scales)):
+            raise ValueError("copies, weight_decay and lr_scale need one entry per tensor")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self.device = self.params[0].device
+        for p, c in zip(self.params, self.copies):
+            if p.dtype != torch.float32 or not p.is_cuda or p.device != self.device or not p.is_contiguous():
+                raise ValueError("weights must be contiguous float32 tensors of one CUDA device")
+            if c is not None and (c.dtype not in (torch.float16, torch.bfloat16) or c.shape != p.shape
+                                  or c.device != self.device or not c.is_contiguous()):
+                raise ValueError("copies must be contiguous float16 or bfloat16 tensors of their weights' shapes")
+        self.lr, self.betas, self.eps, self.max_norm, self.seed, self.steps = lr, tuple(betas), eps, max_norm, seed, 0
+        self.offsets, total = [], 0
+        for p in self.params:
+            self.offsets.append(total)
+            total += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
+        self.m, self.v = torch.zeros(total, device=self.device), torch.zeros(total, device=self.device)
+        self.m_scale = self.v_scale = None
+        if state_bits == 8:
+            self.m, self.v = self.m.to(torch.float8_e4m3fn), self.v.to(torch.float8_e4m3fn)
+            self.m_scale = torch.ones(total // ADAMW_BLOCK, device=self.device)
+            self.v_scale = torch.ones(total // ADAMW_BLOCK, device=self.device)
+        self._dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        table = (AdamWTensor * count)()
+        size = self.m.element_size()
+        for t, p, c, at, decay, scale in zip(table, self.params, self.copies, self.offsets, decays, scales):
+            t.param, t.n, t.weight_decay, t.lr_scale = p.data_ptr(), p.numel(), decay, scale
+            t.m, t.v = self.m.data_ptr() + at * size, self.v.data_ptr() + at * size
+            if state_bits == 8:
+                t.m_scale = self.m_scale.data_ptr() + at // ADAMW_BLOCK * 4
+                t.v_scale = self.v_scale.data_ptr() + at // ADAMW_BLOCK * 4
+            if c is not None:
+                t.copy, t.copy_dtype = c.data_ptr(), self._dtypes[c.dtype]
+        _check(_lib.gz_adamw_create(table, count, state_bits, self.device.index, C.byref(self._plan)))
+        self._grads, self._kinds, self._cfg = (_vp * count)(), (C.c_int32 * count)(), AdamWConfig()
+
+    def close(self) -> None:
+        if self._plan:
+            _lib.gz_adamw_destroy(self._plan)
+            self._plan = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001
+            pass
+
+    def step(self, grads=None, grad_scale=1.0, stream=None):
+        """One step with `grads` (contiguous tensors of the weights' shapes in
+        float32, float16 or bfloat16, None where a weight stays as it is; the
+        weights' .grad by default), each multiplied by grad_scale.  Returns
+        their global norm (a float32 device tensor) with max_norm > 0, else
+        None."""
+        import torch
+        if grads is None:
+            grads = [p.grad for p in self.params]
+        if len(grads) != len(self.params):
+            raise ValueError("grads needs one entry per tensor")
+        for k, (g, p) in enumerate(zip(grads, self.params)):
+            if g is None:
+                self._grads[k] = None
+                continue
+            kind = self._dtypes.get(g.dtype)
+            if kind is None or g.shape != p.shape or g.device != self.device or not g.is_contiguous():
+                raise ValueError("gradients must be contiguous tensors of their weights' shapes in float32, float16 "
+                                 "or bfloat16")
+            self._grads[k], self._kinds[k] = g.data_ptr(), kind
+        norm = torch.empty((), device=self.device) if self.max_norm > 0 else None
+        c = self._cfg
+        c.lr, (c.beta1, c.beta2), c.eps = self.lr, self.betas, self.eps
+        c.max_norm, c.grad_scale, c.step, c.seed = self.max_norm, grad_scale, self.steps + 1, self.seed
+        with _On(self.device):
+            _check(_lib.gz_adamw_step(self._plan, self._grads, self._kinds, C.byref(c), _dev(norm), _stream(stream)))
+        self.steps += 1
+        return norm
 
 
 # ---- reference-layout shim (include/graphzero_b200_compat.h) ----

@@ -386,6 +386,120 @@ gz_status gz_train_batch_indices(int64_t n, const gz_train_config* cfg, int epoc
  * heads, blocks 9 down to 0, the stem.)  Host only. */
 gz_status gz_train_bucket_range(int game, int k, size_t* offset, size_t* count);
 
+/* ---- policies of the caller's own: drawing actions, loss, optimiser -------
+ * No counterpart in the reference, which draws moves from visit counts only
+ * (mcts/mcts.cu:40-66) and trains its own networks only.  For policies that
+ * live elsewhere (a torch model's logits, the logarithm of a net's pi): rows
+ * of scores with the legal moves as a mask, actions drawn from them, the
+ * policy loss with its gradient on the same rows, and an optimiser step over
+ * the model's tensors.  All pointers are device pointers of the current
+ * device unless said otherwise; calls are asynchronous on `stream` (a
+ * cudaStream_t; NULL = the legacy default stream), can be captured in a
+ * graph, and allocate nothing. */
+typedef enum { GZ_F32 = 0, GZ_F16 = 1, GZ_BF16 = 2 } gz_dtype;
+#define GZ_POLICY_MAX_ACTIONS 262144
+/* Rows of action scores.  A visible action is one whose mask byte is not 0;
+ * what lies at the others (infinities and NaN too) has no influence.  Strides
+ * are in elements from row to row, 0 for one row that all share; any
+ * alignment of the elements' own type is taken. */
+typedef struct {
+  const void* logits;    /* [rows][actions] of dtype */
+  const uint8_t* mask;   /* [rows][actions], NULL: every action is visible */
+  int64_t logits_stride;
+  int64_t mask_stride;
+  int64_t rows;          /* 0 .. 2^31 - 1 */
+  int32_t actions;       /* 1 .. GZ_POLICY_MAX_ACTIONS */
+  int32_t dtype;         /* gz_dtype */
+} gz_policy_rows;
+/* How actions are drawn.  Each setting is one value for all rows, or a device
+ * array [rows] where its pointer is not NULL (values out of range are then
+ * taken as the nearest end of the range).
+ *   temperature  >= 0; 0 picks the best action
+ *   top_k        only the k best actions; 0: all
+ *   top_p        of those, the best ones until their share reaches top_p; 1: all
+ *   min_p        of those, the ones at least min_p times as likely as the best; 0: all */
+typedef struct {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float *d_temperature, *d_top_p, *d_min_p;
+  const int32_t* d_top_k;
+} gz_sample_config;
+/* One action per row, drawn with the caller's random numbers: over the
+ * visible actions with a score above -inf (NaN counts as -inf, +inf as the
+ * largest float), ordered by score and at equal scores by index,
+ *   d_j = (x_j - max x) / temperature,  p_j ~ exp(d_j) over the kept ones,
+ *   action = the kept j with the largest d_j + noise[j], the lowest on ties,
+ *   logp   = log p of that action among the kept ones (0 at temperature 0).
+ * noise [rows][actions] holds standard Gumbel numbers, -log(-log u), which
+ * makes the action a draw from p (a noise of NaN counts as -inf); NULL: no
+ * noise, the best action.  A row with nothing visible: action -1, logp 0.
+ * Sums are exact integers, so a row's result does not depend on the batch it
+ * is in.  d_logp may be NULL. */
+gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sample_config* cfg, const float* d_noise,
+                           int64_t noise_stride, int32_t* d_action, float* d_logp, void* stream);
+/* Cross-entropy of the policy p = softmax(logits) over the visible actions,
+ * and its gradient, in one pass:
+ *   loss_i = w_i * -sum_j t_ij log p_ij
+ *   grad_ij = grad_scale * w_i * (p_ij sum_k t_ik - t_ij),  0 where masked
+ * Targets are either d_target [rows][actions] (fp32, any non-negative or
+ * signed amounts; those at masked actions are ignored, and an amount of 0
+ * adds nothing even where log p is -inf) or d_label [rows] (t = 1 at the
+ * label; a label outside the row or at a masked action makes t = 0); exactly
+ * one of the two is given.  d_weight [rows] holds w (NULL: 1), an advantage
+ * for instance.  A row without a visible score above -inf: loss 0, gradient
+ * 0.  A NaN or +inf among the visible scores makes the row's loss and
+ * gradient NaN.  d_loss [rows] fp32; d_grad [rows][actions] of the logits'
+ * dtype, NULL for the loss alone, and it overlaps no input.  fp32 inside,
+ * in an order that depends on the row's length and alignment only. */
+gz_status gz_policy_loss(const gz_policy_rows* rows, const float* d_target, int64_t target_stride,
+                         const int32_t* d_label, const float* d_weight, float grad_scale, float* d_loss, void* d_grad,
+                         int64_t grad_stride, void* stream);
+
+/* AdamW (decoupled weight decay) over many tensors in one launch.  Per weight,
+ * with g the gradient times grad_scale and the clipping factor:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * in fp32, each operation rounded by itself.  States of 32 bits: m and v as
+ * fp32 [n].  States of 8 bits: m and sqrt(v) as 8-bit floats (4 exponent and
+ * 3 mantissa bits, no infinities: the "e4m3fn" format) [n rounded up to
+ * GZ_ADAMW_BLOCK], each block of GZ_ADAMW_BLOCK with an fp32 power of two as
+ * its scale that brings its largest magnitude into (224, 448]; the rounding
+ * is stochastic by a hash of (seed, t, index), since a step of 1 - beta2 is
+ * far below half a grain of the format and would never land, and a positive
+ * root never becomes 0.  The update itself uses m and v before they are
+ * rounded. */
+#define GZ_ADAMW_BLOCK 256
+typedef struct {
+  float* param;          /* [n] fp32 weights */
+  void* copy;            /* [n] 16-bit working copy written with every step, NULL: none */
+  void *m, *v;           /* states (8 bits: 16-byte aligned) */
+  float *m_scale, *v_scale; /* 8 bits: [ceil(n / GZ_ADAMW_BLOCK)]; 32 bits: unused */
+  int64_t n;
+  double weight_decay;   /* decay of this tensor */
+  double lr_scale;       /* its learning rate over the step's */
+  int32_t copy_dtype;    /* GZ_F16 or GZ_BF16 where there is a copy */
+} gz_adamw_tensor;
+typedef struct {
+  double lr, beta1, beta2, eps;
+  double max_norm;       /* > 0: gradients are scaled down to this global norm */
+  float grad_scale;      /* factor on every gradient (1 / the loss scale, say) */
+  int64_t step;          /* t, from 1 */
+  uint64_t seed;         /* of the 8-bit rounding */
+} gz_adamw_config;
+typedef struct gz_adamw gz_adamw;
+/* A plan over `count` tensors of `device` (host array; the buffers stay the
+ * caller's).  state_bits 8 or 32.  Allocates and synchronises. */
+gz_status gz_adamw_create(const gz_adamw_tensor* tensors, int count, int state_bits, int device, gz_adamw** out);
+gz_status gz_adamw_destroy(gz_adamw* a);
+/* One step.  d_grads: host array of `count` device pointers [n], NULL for a
+ * tensor that has no gradient in this step (it stays as it is); grad_dtypes:
+ * host array of their gz_dtype, NULL: all GZ_F32.  d_norm (may be NULL; one
+ * float on the device) receives the global 2-norm of the scaled gradients.
+ * The norm is taken when max_norm > 0 or d_norm is given, in a fixed order.
+ * Steps of one plan must be ordered (one stream, or events between them). */
+gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, const int32_t* grad_dtypes,
+                        const gz_adamw_config* cfg, float* d_norm, void* stream);
+
 /* ---- allocation-free leaf evaluation --------------------------------------
  * No counterpart in the reference.  For callers that may not allocate device
  * memory (a plugin inside a host application that fixes the device-memory
