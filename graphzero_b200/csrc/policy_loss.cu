@@ -1,60 +1,9 @@
-// Drawing actions from rows of policy scores, and the policy loss with its
-// gradient (gz_policy_sample, gz_policy_loss).  One block per row.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-#include <float.h>
-#include <math.h>
-#include <stdint.h>
-
-#include "gz_internal.h"
-#include "gz_sm100.h"
+// The policy loss and its gradient (gz_policy_loss).
+#include "gz_policy.h"
 
 namespace gz {
+namespace policy {
 namespace {
-
-constexpr int kThreads = 256;
-
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-// 16 bytes of floats rounded to T.
-template <typename T> __device__ __forceinline__ uint4 pack(const float* x);
-template <> __device__ __forceinline__ uint4 pack<float>(const float* x) {
-  const float4 v = make_float4(x[0], x[1], x[2], x[3]);
-  return *(const uint4*)&v;
-}
-template <> __device__ __forceinline__ uint4 pack<__half>(const float* x) {
-  uint4 v;
-  for (int k = 0; k < 4; ++k) ((__half2*)&v)[k] = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
-  return v;
-}
-template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float* x) {
-  uint4 v;
-  for (int k = 0; k < 4; ++k) ((__nv_bfloat162*)&v)[k] = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
-  return v;
-}
-template <> __device__ __forceinline__ float from_f32(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
-
-struct RowArgs {
-  const void* logits;
-  const uint8_t* mask;
-  int64_t logits_stride, mask_stride;
-  int actions;
-};
-
-struct SampleArgs {
-  RowArgs rows;
-  gz_sample_config cfg;
-  const float* noise;
-  int64_t noise_stride;
-  int32_t* action;
-  float* logp;
-};
 
 struct LossArgs {
   RowArgs rows;
@@ -73,145 +22,6 @@ struct LossArgs {
 constexpr int64_t kRowsPerLaunch = 1 << 26;  // rows x 16 blocks stay a valid grid
 constexpr int kSharedPerSM = 227 * 1024;
 constexpr int kSliceVecs = 6400;             // 16-byte vectors of a block's slice of a row: two blocks fit an SM
-
-struct MaxOp {
-  template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; }
-};
-struct SumOp {
-  template <typename V> __device__ V operator()(V a, V b) const { return a + b; }
-};
-
-// Every thread gets the reduction of all threads' x, in a fixed order.
-template <typename V, typename Op>
-__device__ V block_reduce(V x, Op op, V* slots) {
-  for (int o = 16; o; o >>= 1) x = op(x, __shfl_xor_sync(~0u, x, o));
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) slots[threadIdx.x / 32] = x;
-  __syncthreads();
-  x = slots[0];
-  for (int w = 1; w < kThreads / 32; ++w) x = op(x, slots[w]);
-  return x;
-}
-
-// Order-preserving map of floats to unsigned integers (-0 below +0 is undone
-// by adding 0 first).
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-
-// exp(d) in units of 2^-44 (d <= 0): 2^18 actions sum below 2^63.
-__device__ __forceinline__ uint64_t fixed_weight(float e) { return __float2ull_rd(e * 17592186044416.f); }
-
-// The score of action j, -inf where it takes no part.
-template <typename T>
-__device__ __forceinline__ float score(const T* x, const uint8_t* mask, int j) {
-  if (mask && !mask[j]) return -INFINITY;
-  const float v = to_f32(x[j]);
-  return v > -INFINITY ? fminf(v, FLT_MAX) : -INFINITY;
-}
-
-// Rank order as one number: higher scores first, at equal scores lower indices.
-__device__ __forceinline__ uint64_t rank_key(float x, int j) {
-  return (uint64_t)order_key(x) << 18 | (uint64_t)(GZ_POLICY_MAX_ACTIONS - 1 - j);
-}
-
-// The threshold of top_k and of top_p is the rank key of the last action kept,
-// found by bisection on the key's 50 bits: each step counts (or weighs) what
-// lies at or above the middle.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
-  __shared__ float sf[kThreads / 32];
-  __shared__ uint64_t su[kThreads / 32];
-  const int64_t row = blockIdx.x;
-  const int A = a.rows.actions;
-  const T* x = (const T*)a.rows.logits + row * a.rows.logits_stride;
-  const uint8_t* mask = a.rows.mask ? a.rows.mask + row * a.rows.mask_stride : nullptr;
-  const float temperature = fminf(a.cfg.d_temperature ? a.cfg.d_temperature[row] : a.cfg.temperature, FLT_MAX);
-  const float top_p = a.cfg.d_top_p ? a.cfg.d_top_p[row] : a.cfg.top_p;
-  const float min_p = fminf(a.cfg.d_min_p ? a.cfg.d_min_p[row] : a.cfg.min_p, 1.f);
-  const int top_k = a.cfg.d_top_k ? a.cfg.d_top_k[row] : a.cfg.top_k;
-  const bool greedy = !(temperature > 0.f);
-
-  float top = -INFINITY;
-  for (int j = threadIdx.x; j < A; j += kThreads) top = fmaxf(top, score(x, mask, j));
-  top = block_reduce(top, MaxOp(), sf);
-  if (top == -INFINITY) {
-    if (threadIdx.x == 0) {
-      a.action[row] = -1;
-      if (a.logp) a.logp[row] = 0.f;
-    }
-    return;
-  }
-  auto depth = [&](float v) { return __fdiv_rn(v - top, temperature); };
-  uint64_t last = 0;  // rank key of the last action kept
-  if (greedy || top_k == 1 || !(top_p > 0.f)) {
-    uint64_t best = 0;
-    for (int j = threadIdx.x; j < A; j += kThreads) {
-      const float v = score(x, mask, j);
-      if (v > -INFINITY) best = MaxOp()(best, rank_key(v, j));
-    }
-    last = block_reduce(best, MaxOp(), su);
-  } else {
-    // the largest key with at least top_k keys at or above it
-    if (top_k > 0 && top_k < A) {
-      for (int bit = 49; bit >= 0; --bit) {
-        const uint64_t mid = last | 1ull << bit;
-        uint64_t c = 0;
-        for (int j = threadIdx.x; j < A; j += kThreads) {
-          const float v = score(x, mask, j);
-          c += v > -INFINITY && rank_key(v, j) >= mid;
-        }
-        if (block_reduce(c, SumOp(), su) >= (uint64_t)top_k) last = mid;
-      }
-    }
-    if (top_p < 1.f) {
-      uint64_t z = 0;
-      for (int j = threadIdx.x; j < A; j += kThreads) {
-        const float v = score(x, mask, j);
-        if (v > -INFINITY && rank_key(v, j) >= last) z += fixed_weight(expf(depth(v)));
-      }
-      const double goal = (double)top_p * (double)block_reduce(z, SumOp(), su);
-      // the largest key with at least the goal's weight at or above it
-      uint64_t cut = 0;
-      for (int bit = 49; bit >= 0; --bit) {
-        const uint64_t mid = cut | 1ull << bit;
-        uint64_t s = 0;
-        for (int j = threadIdx.x; j < A; j += kThreads) {
-          const float v = score(x, mask, j);
-          if (v > -INFINITY && rank_key(v, j) >= mid) s += fixed_weight(expf(depth(v)));
-        }
-        if ((double)block_reduce(s, SumOp(), su) >= goal) cut = mid;
-      }
-      last = MaxOp()(last, cut);
-    }
-  }
-  // the draw among the kept actions, and their weight
-  const float* noise = a.noise ? a.noise + row * a.noise_stride : nullptr;
-  uint64_t best = 0, z = 0;
-  for (int j = threadIdx.x; j < A; j += kThreads) {
-    const float v = score(x, mask, j);
-    if (v == -INFINITY || rank_key(v, j) < last) continue;
-    float s = 0.f;
-    if (!greedy) {
-      const float d = depth(v), e = expf(d);
-      if (e < min_p) continue;
-      z += fixed_weight(e);
-      s = d + (noise ? noise[j] : 0.f);
-      if (!(s >= -INFINITY)) s = -INFINITY;
-    }
-    best = MaxOp()(best, rank_key(s, j));
-  }
-  z = block_reduce(z, SumOp(), su);
-  best = block_reduce(best, MaxOp(), su);
-  if (threadIdx.x == 0) {
-    const int j = GZ_POLICY_MAX_ACTIONS - 1 - (int)(best & (GZ_POLICY_MAX_ACTIONS - 1));
-    a.action[row] = j;
-    if (a.logp) a.logp[row] = greedy ? 0.f : depth(score(x, mask, j)) - logf((float)((double)z * 0x1p-44));
-  }
-}
-
-// ---- loss -------------------------------------------------------------------
 
 // What a part of a row contributes: m the largest visible score, z the sum of
 // exp(x - m), mass and cross the sums of t and t (x - m).  With m = -inf
@@ -250,12 +60,6 @@ __device__ __forceinline__ Part merge(Part a, Part b) {
   return {m, a.z + b.z, a.mass + b.mass, a.cross + b.cross};
 }
 
-// Maximum over the warp's lanes (no lane holds a NaN).
-__device__ __forceinline__ float warp_max(float x) {
-  const uint32_t k = __reduce_max_sync(~0u, order_key(x));
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-
 // Sums over the warp's lanes, of parts relative to the same m.
 template <bool kDense>
 __device__ __forceinline__ Part warp_sum(Part p) {
@@ -275,21 +79,6 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 // Ends a group of copies; waits for all of this thread's groups but the last kLeft.
 __device__ __forceinline__ void end_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
-
-// V scores of a vector as floats.
-template <typename T> __device__ __forceinline__ void unpack(uint4 raw, float* x);
-template <> __device__ __forceinline__ void unpack<float>(uint4 raw, float* x) {
-  for (int k = 0; k < 4; ++k) x[k] = __uint_as_float((&raw.x)[k]);
-}
-template <> __device__ __forceinline__ void unpack<__half>(uint4 raw, float* x) {
-  for (int k = 0; k < 4; ++k) *(float2*)(x + 2 * k) = __half22float2(((const __half2*)&raw)[k]);
-}
-template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint4 raw, float* x) {
-  for (int k = 0; k < 4; ++k) {  // a bf16 is the upper half of its float
-    x[2 * k] = __uint_as_float((&raw.x)[k] << 16);
-    x[2 * k + 1] = __uint_as_float((&raw.x)[k] & 0xffff0000u);
-  }
-}
 
 // Visibility of V actions, a bit each.
 template <int V> __device__ __forceinline__ uint32_t visible_bits(const uint8_t* mask, bool aligned) {
@@ -446,30 +235,6 @@ __device__ __forceinline__ void add_vector(Part& p, float2& z, uint4 raw, uint32
         p.cross += t[k] * (f[k] - ref);
       }
   }
-}
-
-// Maximum of a vector's visible scores and m.
-template <bool kMasked, typename T>
-__device__ __forceinline__ float max_vector(float m, uint4 raw, uint32_t bits) {
-  constexpr int V = 16 / (int)sizeof(T);
-  float f[V];
-  unpack<T>(raw, f);
-#pragma unroll
-  for (int k = 0; k < V; ++k)
-    if (!kMasked || (bits >> k & 1)) m = fmaxf(m, f[k]);
-  return m;
-}
-template <typename T2> __device__ __forceinline__ T2 max_pairs(uint4 raw) {
-  const T2* p = (const T2*)&raw;
-  return __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
-}
-template <> __device__ __forceinline__ float max_vector<false, __half>(float m, uint4 raw, uint32_t) {
-  const float2 f = __half22float2(max_pairs<__half2>(raw));
-  return fmaxf(m, fmaxf(f.x, f.y));
-}
-template <> __device__ __forceinline__ float max_vector<false, __nv_bfloat16>(float m, uint4 raw, uint32_t) {
-  const float2 f = __bfloat1622float2(max_pairs<__nv_bfloat162>(raw));
-  return fmaxf(m, fmaxf(f.x, f.y));
 }
 
 // Short rows: a warp each, four a block, scores in registers.
@@ -977,53 +742,12 @@ cudaError_t launch_loss(LossArgs a, int64_t rows, cudaStream_t stream) {
   return e;
 }
 
-gz_status bad(const char* who, const char* what) { return set_last_error(GZ_ERR_INVALID_ARG, "%s: %s", who, what); }
-
-gz_status check_rows(const gz_policy_rows* r, const char* who) {
-  if (!r) return bad(who, "null argument");
-  if (r->rows < 0 || r->rows > INT32_MAX) return bad(who, "rows must be 0 .. 2^31 - 1");
-  if (r->actions < 1 || r->actions > GZ_POLICY_MAX_ACTIONS)
-    return set_last_error(GZ_ERR_INVALID_ARG, "%s: actions must be 1 .. %d", who, GZ_POLICY_MAX_ACTIONS);
-  if (r->dtype < GZ_F32 || r->dtype > GZ_BF16) return bad(who, "bad dtype");
-  if (r->logits_stride < 0 || r->mask_stride < 0) return bad(who, "negative stride");
-  if (r->rows > 0 && !r->logits) return bad(who, "null logits");
-  return GZ_OK;
-}
-
-RowArgs row_args(const gz_policy_rows* r) {
-  return {r->logits, r->mask, r->logits_stride, r->mask_stride, r->actions};
-}
-
-gz_status launched(const char* who) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? GZ_OK : set_last_error(GZ_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
-}
-
 }  // namespace
+}  // namespace policy
 }  // namespace gz
 
 using namespace gz;
-
-extern "C" gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sample_config* cfg, const float* d_noise,
-                                      int64_t noise_stride, int32_t* d_action, float* d_logp, void* stream) {
-  const char* who = "gz_policy_sample";
-  if (gz_status s = check_rows(rows, who)) return s;
-  if (!cfg) return bad(who, "null argument");
-  if (!cfg->d_temperature && !(cfg->temperature >= 0.f)) return bad(who, "temperature must be at least 0");
-  if (!cfg->d_top_k && cfg->top_k < 0) return bad(who, "top_k must be at least 0");
-  if (!cfg->d_top_p && !(cfg->top_p >= 0.f && cfg->top_p <= 1.f)) return bad(who, "top_p must be 0 .. 1");
-  if (!cfg->d_min_p && !(cfg->min_p >= 0.f && cfg->min_p <= 1.f)) return bad(who, "min_p must be 0 .. 1");
-  if (noise_stride < 0) return bad(who, "negative stride");
-  if (rows->rows == 0) return GZ_OK;
-  if (!d_action) return bad(who, "null actions");
-  const SampleArgs a{row_args(rows), *cfg, d_noise, noise_stride, d_action, d_logp};
-  const cudaStream_t s = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)rows->rows;
-  if (rows->dtype == GZ_F32) sample_kernel<float><<<grid, kThreads, 0, s>>>(a);
-  else if (rows->dtype == GZ_F16) sample_kernel<__half><<<grid, kThreads, 0, s>>>(a);
-  else sample_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
-  return launched(who);
-}
+using namespace gz::policy;
 
 extern "C" gz_status gz_policy_loss(const gz_policy_rows* rows, const float* d_target, int64_t target_stride,
                                     const int32_t* d_label, const float* d_weight, float grad_scale, float* d_loss,

@@ -1,0 +1,620 @@
+// Drawing actions from rows of policy scores (gz_policy_sample).
+//
+// A row's order is that of its rank keys: the score's bits in an order-
+// preserving form, then the index, so that no two are alike, and the kept
+// actions of top_k and top_p are those from some rank key on.  Few candidates
+// are put into a list in shared memory and sorted; which way a row gets there:
+//  - Masked rows list their visible actions (16 mask bytes at a time; scores are
+//    read only where something is visible), and rows of at most kList actions
+//    list all of them.
+//  - Longer rows are read once for their best score and, where top_p needs it,
+//    their sum of exponentials.  The K-th largest of the threads' best scores
+//    has at least K actions at or above it: those are listed in a second pass,
+//    from the caches.  top_k takes K = top_k.  For top_p, K is half of the
+//    threads, and the list is enough if it reaches the share wanted.
+//  - Where it is not (flat rows, a large top_k), a histogram over the scores
+//    finds the bin that the last kept action lies in, and only that bin is
+//    listed and sorted; if a bin overflows the list (equal scores), the last
+//    rank key is found by bisection.
+// The draw is an argmax over the kept actions; noise is read for these alone.
+//
+// Weights exp(d) of listed actions are summed as integers in units of 2^-44, so
+// that neither the list's order nor the atomics' matters; sums over whole rows
+// are 32-bit floats in an order given by the row's length and alignment.
+#include "gz_policy.h"
+
+namespace gz {
+namespace policy {
+namespace {
+
+struct SampleArgs {
+  RowArgs rows;
+  gz_sample_config cfg;
+  const float* noise;
+  int64_t noise_stride;
+  int32_t* action;
+  float* logp;
+  int64_t first_row, end_row;  // of this launch
+};
+
+constexpr int kList = 2048;         // keys a block's list holds
+constexpr int kWarpRow = 256;       // actions of a row that a warp takes
+constexpr int kBins = 1024;         // of the histogram, which the list's memory holds
+constexpr int kSampleThreads = 512;  // most threads of a block
+constexpr int64_t kRowsPerLaunch = 1 << 28;
+
+// exp(d) in units of 2^-44 (d <= 0): 2^18 actions sum below 2^63.
+__device__ __forceinline__ uint64_t fixed_weight(float e) { return __float2ull_rd(e * 0x1p44f); }
+
+// Rank order as one number: higher scores first, at equal scores lower indices.
+__device__ __forceinline__ uint64_t rank_key(float x, int j) {
+  return (uint64_t)order_key(x) << 18 | (uint64_t)(GZ_POLICY_MAX_ACTIONS - 1 - j);
+}
+__device__ __forceinline__ int key_index(uint64_t k) {
+  return GZ_POLICY_MAX_ACTIONS - 1 - (int)(k & (GZ_POLICY_MAX_ACTIONS - 1));
+}
+__device__ __forceinline__ float key_score(uint64_t k) { return key_value((uint32_t)(k >> 18)); }
+
+// The threads that share a row: a warp, or the block.
+template <bool kWarp> struct Team {
+  uint64_t* slots;  // a word per warp
+  int tid, n;
+  __device__ void sync() const {
+    if (kWarp) __syncwarp();
+    else __syncthreads();
+  }
+  template <typename V, typename Op> __device__ V reduce(V x, Op op) const {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = op(x, __shfl_xor_sync(~0u, x, o));
+    if (kWarp) return x;
+    V* s = (V*)slots;
+    __syncthreads();
+    if (tid % 32 == 0) s[tid / 32] = x;
+    __syncthreads();
+    x = s[0];
+    for (int w = 1; w < n / 32; ++w) x = op(x, s[w]);
+    return x;
+  }
+  template <typename V> __device__ V max(V x) const {
+    return reduce(x, [](V a, V b) { return a > b ? a : b; });
+  }
+  template <typename V> __device__ V sum(V x) const {
+    return reduce(x, [](V a, V b) { return a + b; });
+  }
+  // Sum of the x of the threads before this one.
+  __device__ uint64_t before(uint64_t x) const {
+    uint64_t up = x;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint64_t y = __shfl_up_sync(~0u, up, o);
+      if (tid % 32 >= o) up += y;
+    }
+    uint64_t sum = up - x;
+    if (kWarp) return sum;
+    __syncthreads();
+    if (tid % 32 == 31) slots[tid / 32] = up;
+    __syncthreads();
+    for (int w = 0; w < tid / 32; ++w) sum += slots[w];
+    return sum;
+  }
+};
+
+template <typename T> struct Row {
+  static constexpr int V = 16 / (int)sizeof(T);
+  const T* x;
+  const uint8_t* mask;
+  const float* noise;
+  int actions, head, vecs, ends;  // scores before the first 16-byte boundary, vectors, scores beside them
+
+  __device__ Row(const SampleArgs& a, int64_t row) {
+    actions = a.rows.actions;
+    x = (const T*)a.rows.logits + row * a.rows.logits_stride;
+    mask = a.rows.mask ? a.rows.mask + row * a.rows.mask_stride : nullptr;
+    noise = a.noise ? a.noise + row * a.noise_stride : nullptr;
+    head = min(actions, (int)(-(uintptr_t)x & 15) / (int)sizeof(T));
+    vecs = (actions - head) / V;
+    ends = actions - vecs * V;
+  }
+  __device__ int end_index(int i) const { return i < head ? i : actions - ends + i; }
+  __device__ uint4 vector(int v) const { return __ldg((const uint4*)(x + head) + v); }
+};
+
+// f(j, score) for this thread's share of the visible actions.
+template <typename T, typename F> __device__ __forceinline__ void each(const Row<T>& r, int tid, int n, F f) {
+  auto one = [&](int j, float v) {
+    if (v > -INFINITY) f(j, fminf(v, FLT_MAX));  // a NaN counts as -inf
+  };
+  if (r.mask) {
+    const int head = min(r.actions, (int)(-(uintptr_t)r.mask & 15));
+    const int groups = (r.actions - head) / 16, ends = r.actions - groups * 16;
+    const int ej = tid < head ? tid : r.actions - ends + tid;
+    if (tid < ends && r.mask[ej]) one(ej, to_f32(r.x[ej]));
+#pragma unroll 2
+    for (int u = tid; u < groups; u += n) {
+      const uint4 w = __ldg((const uint4*)(r.mask + head) + u);
+      if (!(w.x | w.y | w.z | w.w)) continue;
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k)
+        for (uint32_t bits = __vcmpne4(k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w, 0) & 0x01010101u; bits; bits &= bits - 1) {
+          const int j = head + u * 16 + k * 4 + (__ffs(bits) - 1) / 8;
+          one(j, to_f32(r.x[j]));
+        }
+    }
+  } else {
+    if (tid < r.ends) one(r.end_index(tid), to_f32(r.x[r.end_index(tid)]));
+    for (int v = tid; v < r.vecs; v += n) {
+      float x[Row<T>::V];
+      unpack<T>(r.vector(v), x);
+#pragma unroll
+      for (int k = 0; k < Row<T>::V; ++k) one(r.head + v * Row<T>::V + k, x[k]);
+    }
+  }
+}
+
+struct Filters {
+  float temperature, top_p, min_p;
+  int top_k;
+  bool greedy;  // the best action alone
+
+  __device__ Filters(const gz_sample_config& c, int64_t row) {
+    temperature = fminf(c.d_temperature ? c.d_temperature[row] : c.temperature, FLT_MAX);
+    top_p = c.d_top_p ? c.d_top_p[row] : c.top_p;
+    min_p = fminf(c.d_min_p ? c.d_min_p[row] : c.min_p, 1.f);
+    top_k = c.d_top_k ? c.d_top_k[row] : c.top_k;
+    greedy = !(temperature > 0.f) || top_k == 1 || !(top_p > 0.f);
+  }
+  __device__ float depth(float x, float top) const { return temperature == 1.f ? x - top : __fdiv_rn(x - top, temperature); }
+};
+
+__device__ __forceinline__ void answer(const SampleArgs& a, int64_t row, int action, float logp) {
+  a.action[row] = action;
+  if (a.logp) a.logp[row] = logp;
+}
+
+// The best of a row's noisy scores so far, and the kept weight.
+struct Draw {
+  uint64_t best = 0, weight = 0;
+  __device__ void add(const Filters& f, float top, float x, int j, const float* noise) {
+    const float d = f.depth(x, top), e = expf(d);
+    if (e < f.min_p) return;
+    weight += fixed_weight(e);
+    const float s = noise ? d + noise[j] : d;
+    const uint64_t key = rank_key(s >= -INFINITY ? s : -INFINITY, j);
+    if (key > best) best = key;
+  }
+  template <typename T, bool kWarp>
+  __device__ void finish(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T>& r, const Filters& f, float top) {
+    weight = team.sum(weight);
+    best = team.max(best);
+    if (team.tid == 0) {
+      const int j = key_index(best);
+      answer(a, row, j, f.depth(fminf(to_f32(r.x[j]), FLT_MAX), top) - logf((float)((double)weight * 0x1p-44)));
+    }
+  }
+};
+
+// Sorts keys[0 .. size) downwards; the memory behind them up to a power of two is used.
+template <bool kWarp> __device__ void sort_keys(const Team<kWarp>& team, uint64_t* keys, int size) {
+  int p = 2;
+  while (p < size) p *= 2;
+  for (int i = size + team.tid; i < p; i += team.n) keys[i] = 0;
+  team.sync();
+  for (int k = 2; k <= p; k *= 2)
+    for (int h = k / 2; h; h /= 2) {
+      for (int i = team.tid; i < p / 2; i += team.n) {
+        const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
+        const uint64_t x = keys[lo], y = keys[hi];
+        if ((x < y) == ((lo & k) == 0)) {
+          keys[lo] = y;
+          keys[hi] = x;
+        }
+      }
+      team.sync();
+    }
+}
+
+// How many of the sorted keys[0 .. m) have less than `goal` before them, where
+// `above` lies before the first and a key counts its weight, or 1.
+template <bool kWeights, bool kWarp>
+__device__ int keys_before(const Team<kWarp>& team, const uint64_t* keys, int m, const Filters& f, float top, double goal,
+                           uint64_t above, uint64_t* total) {
+  const int per = (m + team.n - 1) / team.n, lo = min(m, team.tid * per), hi = min(m, lo + per);
+  auto weight = [&](int i) { return kWeights ? fixed_weight(expf(f.depth(key_score(keys[i]), top))) : 1ull; };
+  uint64_t mine = 0;
+  for (int i = lo; i < hi; ++i) mine += weight(i);
+  uint64_t sum = above + team.before(mine);
+  if (total) {
+    *total = team.max(sum + mine);
+    if (goal < 0) goal = -goal * (double)*total;  // a share of the keys' own weight
+  }
+  int c = 0;
+  for (int i = lo; i < hi && (double)sum < goal; ++i, ++c) sum += weight(i);
+  return team.sum(c);
+}
+
+// Draws from a list of a row's best actions: all that can be kept.  size: keys
+// in memory, of which `count` are not 0.  row_weight < 0: the list is the whole
+// row or top_k's; else the row's weight, and false comes back if the list does
+// not reach top_p's share of it.
+template <typename T, bool kWarp>
+__device__ bool draw_from_list(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T>& r, const Filters& f,
+                               uint64_t* keys, int size, int count, float top, double row_weight) {
+  if ((f.top_k > 0 && f.top_k < count) || f.top_p < 1.f) {
+    sort_keys(team, keys, size);
+    size = f.top_k > 0 ? min(count, f.top_k) : count;
+    if (f.top_p < 1.f) {
+      uint64_t total;
+      const double goal = row_weight < 0 ? -(double)f.top_p : f.top_p * row_weight;
+      const int kept = keys_before<true>(team, keys, size, f, top, goal, 0, &total);
+      if (row_weight >= 0 && (double)total < goal) return false;
+      size = max(1, kept);
+    }
+  }
+  Draw d;
+  for (int i = team.tid; i < size; i += team.n)
+    if (keys[i]) d.add(f, top, key_score(keys[i]), key_index(keys[i]), r.noise);
+  d.finish(a, row, team, r, f, top);
+  return true;
+}
+
+// Rows of at most kWarpRow actions: a warp each, four a block.
+template <typename T> __global__ void __launch_bounds__(128) sample_warp_kernel(SampleArgs a) {
+  __shared__ uint64_t lists[4][kWarpRow];
+  const int64_t row = a.first_row + (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
+  if (row >= a.end_row) return;
+  const Team<true> team{nullptr, (int)threadIdx.x % 32, 32};
+  const Row<T> r(a, row);
+  const Filters f(a.cfg, row);
+  uint64_t* keys = lists[threadIdx.x / 32];
+  uint64_t best = 0;
+  int count = 0;
+  for (int j = team.tid; j < r.actions; j += 32) {
+    const float v = r.mask && !r.mask[j] ? -INFINITY : to_f32(r.x[j]);
+    const uint64_t key = v > -INFINITY ? rank_key(fminf(v, FLT_MAX), j) : 0;
+    keys[j] = key;
+    count += key != 0;
+    if (key > best) best = key;
+  }
+  best = team.max(best);
+  count = team.sum(count);
+  team.sync();
+  if (!best || f.greedy) {
+    if (team.tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
+    return;
+  }
+  draw_from_list(a, row, team, r, f, keys, r.actions, count, key_score(best), -1.0);
+}
+
+// The rank key of the last kept action: the largest with at least `goal` (a
+// count, or a weight) at or above it.
+template <bool kWeights, typename T>
+__device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal) {
+  uint64_t last = 0;
+  for (int bit = 49; bit >= 0; --bit) {
+    const uint64_t mid = last | 1ull << bit;
+    uint64_t s = 0;
+    each(r, team.tid, team.n, [&](int j, float x) {
+      if (rank_key(x, j) >= mid) s += kWeights ? fixed_weight(expf(f.depth(x, top))) : 1ull;
+    });
+    if ((double)team.sum(s) >= goal) last = mid;
+  }
+  return last;
+}
+
+// The same through a histogram of kBins bins over the 31 temperatures below the
+// best score (what lies deeper, by bisection if need be).
+template <bool kWeights, typename T>
+__device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal,
+                                              uint64_t* memory, int* counter) {
+  __shared__ uint64_t above;
+  __shared__ int found;
+  unsigned long long* bins = (unsigned long long*)memory;
+  const float scale = kBins / (31.f * f.temperature);
+  auto bin = [&](float x) { return min(kBins - 1, (int)((top - x) * scale)); };  // falls as x rises, weakly
+  team.sync();
+  for (int i = team.tid; i < kBins; i += team.n) bins[i] = 0;
+  if (team.tid == 0) *counter = 0, found = kBins;
+  team.sync();
+  each(r, team.tid, team.n, [&](int, float x) {
+    const unsigned long long w = kWeights ? fixed_weight(expf(f.depth(x, top))) : 1ull;
+    if (w) atomicAdd(&bins[bin(x)], w);
+  });
+  team.sync();
+  const int per = kBins / team.n, lo = team.tid * per;  // n divides kBins or the rest is the last thread's
+  const int hi = team.tid == team.n - 1 ? kBins : lo + per;
+  uint64_t mine = 0;
+  for (int i = lo; i < hi; ++i) mine += bins[i];
+  uint64_t sum = team.before(mine);
+  for (int i = lo; i < hi; ++i) {
+    if ((double)sum < goal && (double)(sum + bins[i]) >= goal) {
+      found = i;
+      above = sum;
+    }
+    sum += bins[i];
+  }
+  team.sync();
+  const int b = found;
+  const uint64_t base = above;
+  if (b == kBins) return last_by_bisection<kWeights>(team, r, f, top, goal);  // out of reach by rounding
+  team.sync();  // the bins have been read
+  each(r, team.tid, team.n, [&](int j, float x) {
+    if (bin(x) == b) {
+      const int at = atomicAdd(counter, 1);
+      if (at < kList) memory[at] = rank_key(x, j);
+    }
+  });
+  team.sync();
+  const int m = *counter;
+  if (m > kList) return last_by_bisection<kWeights>(team, r, f, top, goal);
+  sort_keys(team, memory, m);
+  const int kept = keys_before<kWeights>(team, memory, m, f, top, goal, base, nullptr);
+  const uint64_t last = memory[max(0, kept - 1)];
+  team.sync();
+  return last;
+}
+
+struct Shared {
+  uint64_t slots[kSampleThreads / 32], list[kList];
+  int counter;
+};
+
+// A row whose visible actions do not all fit the list.
+template <typename T, bool kMasked>
+__device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
+  constexpr int V = Row<T>::V;
+  const int64_t row = a.first_row + blockIdx.x;
+  const int tid = threadIdx.x, n = blockDim.x;
+  const Team<false> team{sh.slots, tid, n};
+  const Row<T> r(a, row);
+  const Filters f(a.cfg, row);
+  const bool by_count = f.top_k > 0 && f.top_k < r.actions, by_weight = f.top_p < 1.f;
+  const bool row_weighs = by_weight && !by_count && !f.greedy;
+  const float per_score = 1.44269504f / f.temperature;
+
+  // the thread's best action and, where top_p asks for the row's weight, its
+  // sum of exponentials relative to the best of its first vector
+  uint64_t best = 0;
+  float z = 0.f, z_base = -INFINITY;
+  bool z_fine = false;
+  if (kMasked) {
+    each(r, tid, n, [&](int j, float x) {
+      const uint64_t key = rank_key(x, j);
+      if (key > best) best = key;
+    });
+  } else {
+    float most = -INFINITY, c = 0.f;
+    int where = -1;
+    float2 sum = {0.f, 0.f};
+    constexpr int kAhead = 4;
+    for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
+      uint4 raw[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v0 + i * n < r.vecs) raw[i] = r.vector(v0 + i * n);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (v0 + i * n >= r.vecs) continue;
+        const float m = fminf(max_vector<false, T>(-INFINITY, raw[i], 0), FLT_MAX);
+        if (m > most) {
+          most = m;
+          where = v0 + i * n;
+        }
+        if (row_weighs) {
+          if (z_base == -INFINITY) {
+            z_base = m;
+            c = m == -INFINITY ? 0.f : -m * per_score;
+          }
+          float x[V];
+          unpack<T>(raw[i], x);
+#pragma unroll
+          for (int k = 0; k < V; k += 2) {
+            const float2 y = __ffma2_rn(make_float2(x[k], x[k + 1]), make_float2(per_score, per_score), make_float2(c, c));
+            sum = __fadd2_rn(sum, make_float2(sm100::ex2_approx(y.x), sm100::ex2_approx(y.y)));
+          }
+        }
+      }
+    }
+    if (where >= 0) {
+      float x[V];
+      unpack<T>(r.vector(where), x);
+#pragma unroll
+      for (int k = V - 1; k >= 0; --k)
+        if (fminf(x[k], FLT_MAX) == most) best = rank_key(most, r.head + where * V + k);
+    }
+    // c rounds -z_base per_score; what that leaves on every term is taken out
+    z = (sum.x + sum.y) * (z_base > -INFINITY ? sm100::ex2_approx(-__fmaf_rn(z_base, per_score, c)) : 1.f);
+    if (tid < r.ends) {
+      const float x = fminf(to_f32(r.x[r.end_index(tid)]), FLT_MAX);
+      if (to_f32(r.x[r.end_index(tid)]) > -INFINITY) {
+        const uint64_t key = rank_key(x, r.end_index(tid));
+        if (key > best) best = key;
+        if (z_base == -INFINITY) z_base = x;
+        z += sm100::ex2_approx((x - z_base) * per_score);
+      }
+    }
+    z_fine = z_base == -INFINITY ? z == 0.f : z > 0.f && z < 0x1p64f && fabsf(z_base * per_score) < 1e30f;
+  }
+  const uint64_t mine = best;
+  best = team.max(best);
+  if (!best || f.greedy) {
+    if (tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
+    return;
+  }
+  const float top = key_score(best);
+
+  uint64_t last = 0;  // rank key of the last action that top_k and top_p keep
+  if (by_count || by_weight) {
+    double row_weight = -1.0;
+    if (row_weighs) {
+      if (__syncthreads_and(z_fine)) {
+        z *= z_base > -INFINITY ? sm100::ex2_approx((z_base - top) * per_score) : 0.f;
+      } else {  // beyond what a sum relative to some score holds, or under a mask
+        z = 0.f;
+        each(r, tid, n, [&](int, float x) { z += expf(f.depth(x, top)); });
+      }
+      row_weight = (double)team.sum(z) * 0x1p44;
+    }
+    const int rank = by_count ? f.top_k : n / 2;
+    if (rank <= n) {
+      // the largest number, to 20 bits, that `rank` threads' best scores reach
+      uint32_t reach = 0;
+#pragma unroll 1
+      for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t mid = reach | 1u << bit;
+        if (__syncthreads_count((uint32_t)(mine >> 18) >= mid) >= rank) reach = mid;
+      }
+      if (reach) {
+        const float from = key_value(reach);
+        if (tid == 0) sh.counter = 0;
+        __syncthreads();
+        auto take = [&](int j, float x) {
+          if (x >= from) {
+            const int at = atomicAdd(&sh.counter, 1);
+            if (at < kList) sh.list[at] = rank_key(x, j);
+          }
+        };
+        if (kMasked) {
+          each(r, tid, n, take);
+        } else {
+          if (tid < r.ends) take(r.end_index(tid), fminf(to_f32(r.x[r.end_index(tid)]), FLT_MAX));
+#pragma unroll 4
+          for (int v = tid; v < r.vecs; v += n) {
+            const uint4 raw = r.vector(v);
+            if (max_vector<false, T>(-INFINITY, raw, 0) < from) continue;
+            float x[V];
+            unpack<T>(raw, x);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+              if (x[k] == x[k]) take(r.head + v * V + k, fminf(x[k], FLT_MAX));
+          }
+        }
+        __syncthreads();
+        const int m = sh.counter;
+        if (m <= kList && draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
+      }
+    }
+    if (by_count) last = last_by_bins<false>(team, r, f, top, (double)f.top_k, sh.list, &sh.counter);
+    if (by_weight) {
+      if (by_count) {
+        uint64_t w = 0;
+        each(r, tid, n, [&](int j, float x) {
+          if (rank_key(x, j) >= last) w += fixed_weight(expf(f.depth(x, top)));
+        });
+        row_weight = (double)team.sum(w);
+      }
+      const uint64_t cut = last_by_bins<true>(team, r, f, top, f.top_p * row_weight, sh.list, &sh.counter);
+      if (cut > last) last = cut;
+    }
+  }
+  Draw d;
+  each(r, tid, n, [&](int j, float x) {
+    if (rank_key(x, j) >= last) d.add(f, top, x, j, r.noise);
+  });
+  d.finish(a, row, team, r, f, top);
+}
+
+// A call of its own, so that rows that fit the list do not pay for its registers.
+template <typename T, bool kMasked> __device__ __noinline__ void draw_long_call(const SampleArgs& a, Shared& sh) {
+  draw_long<T, kMasked>(a, sh);
+}
+
+// Rows that are expected to fit the list: masked, or of at most kList actions.
+template <typename T, bool kMasked>
+__global__ void __launch_bounds__(kSampleThreads, 4) sample_list_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ Shared sh;
+  const int64_t row = a.first_row + blockIdx.x;
+  const int tid = threadIdx.x, n = blockDim.x;
+  const Team<false> team{sh.slots, tid, n};
+  const Row<T> r(a, row);
+  uint64_t best = 0;
+  int count = 0;
+  if (kMasked) {
+    if (tid == 0) sh.counter = 0;
+    __syncthreads();
+    each(r, tid, n, [&](int j, float x) {
+      const uint64_t key = rank_key(x, j);
+      if (key > best) best = key;
+      const int at = atomicAdd(&sh.counter, 1);
+      if (at < kList) sh.list[at] = key;
+    });
+  } else {
+    for (int j = tid; j < r.actions; j += n) {
+      const float v = to_f32(r.x[j]);
+      const uint64_t key = v > -INFINITY ? rank_key(fminf(v, FLT_MAX), j) : 0;
+      sh.list[j] = key;
+      count += key != 0;
+      if (key > best) best = key;
+    }
+  }
+  best = team.max(best);
+  const Filters f(a.cfg, row);
+  if (!best || f.greedy) {
+    if (tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
+    return;
+  }
+  count = kMasked ? sh.counter : team.sum(count);
+  const float top = key_score(best);
+  if (count > kList) {
+    __syncthreads();
+    draw_long_call<T, kMasked>(a, sh);
+  } else if (kMasked && count <= 64) {
+    if (tid < 32) draw_from_list(a, row, Team<true>{nullptr, tid, 32}, r, f, sh.list, count, count, top, -1.0);
+  } else {
+    draw_from_list(a, row, team, r, f, sh.list, kMasked ? count : r.actions, count, top, -1.0);
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(kSampleThreads, 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ Shared sh;
+  draw_long<T, false>(a, sh);
+}
+
+template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  for (int64_t first = 0; first < rows && e == cudaSuccess; first += kRowsPerLaunch) {
+    const int64_t n = rows - first < kRowsPerLaunch ? rows - first : kRowsPerLaunch;
+    a.first_row = first;
+    a.end_row = first + n;
+    const int A = a.rows.actions;
+    if (A <= kWarpRow) {
+      sample_warp_kernel<T><<<(unsigned)((n + 3) / 4), 128, 0, stream>>>(a);
+    } else {
+      // two mask groups of 16 a thread, or eight scores, or four vectors
+      const bool masked = a.rows.mask != nullptr, listed = A <= kList;
+      const int units = masked ? A / 32 : listed ? A / 8 : A / (4 * Row<T>::V);
+      const int threads = min(kSampleThreads, max(64, (units + 31) / 32 * 32));
+      auto kernel = masked ? sample_list_kernel<T, true> : listed ? sample_list_kernel<T, false> : sample_long_kernel<T>;
+      kernel<<<(unsigned)n, threads, 0, stream>>>(a);
+    }
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+}  // namespace
+}  // namespace policy
+}  // namespace gz
+
+using namespace gz;
+using namespace gz::policy;
+
+extern "C" gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sample_config* cfg, const float* d_noise,
+                                      int64_t noise_stride, int32_t* d_action, float* d_logp, void* stream) {
+  const char* who = "gz_policy_sample";
+  if (gz_status s = check_rows(rows, who)) return s;
+  if (!cfg) return bad(who, "null argument");
+  if (!cfg->d_temperature && !(cfg->temperature >= 0.f)) return bad(who, "temperature must be at least 0");
+  if (!cfg->d_top_k && cfg->top_k < 0) return bad(who, "top_k must be at least 0");
+  if (!cfg->d_top_p && !(cfg->top_p >= 0.f && cfg->top_p <= 1.f)) return bad(who, "top_p must be 0 .. 1");
+  if (!cfg->d_min_p && !(cfg->min_p >= 0.f && cfg->min_p <= 1.f)) return bad(who, "min_p must be 0 .. 1");
+  if (noise_stride < 0) return bad(who, "negative stride");
+  if (rows->rows == 0) return GZ_OK;
+  if (!d_action) return bad(who, "null actions");
+  const SampleArgs a{row_args(rows), *cfg, d_noise, noise_stride, d_action, d_logp, 0, 0};
+  const cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
+  if (rows->dtype == GZ_F32) e = launch_sample<float>(a, rows->rows, s);
+  else if (rows->dtype == GZ_F16) e = launch_sample<__half>(a, rows->rows, s);
+  else e = launch_sample<__nv_bfloat16>(a, rows->rows, s);
+  return e == cudaSuccess ? GZ_OK : set_last_error(GZ_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}

@@ -433,8 +433,8 @@ typedef struct {
  * noise [rows][actions] holds standard Gumbel numbers, -log(-log u), which
  * makes the action a draw from p (a noise of NaN counts as -inf); NULL: no
  * noise, the best action.  A row with nothing visible: action -1, logp 0.
- * Sums are exact integers, so a row's result does not depend on the batch it
- * is in.  d_logp may be NULL. */
+ * A row's result depends on nothing but the row, its settings and its
+ * alignment: sums are integers or taken in a fixed order.  d_logp may be NULL. */
 gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sample_config* cfg, const float* d_noise,
                            int64_t noise_stride, int32_t* d_action, float* d_logp, void* stream);
 /* Cross-entropy of the policy p = softmax(logits) over the visible actions,
