@@ -27,7 +27,7 @@ namespace gz {
 namespace {
 
 constexpr int kBlock = GZ_ADAMW_BLOCK;
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kStepBlocks = 3;
 constexpr int kPerLane = kBlock / 32;  // elements of a block per lane
 constexpr int kGradsPerLaunch = 416;   // addresses and types per launch (3.7 KB of arguments)
 
@@ -67,29 +67,75 @@ struct StepArgs {
   float* norm;
 };
 
-__device__ __forceinline__ float load_grad(const void* g, int dtype, int64_t i) {
-  if (dtype == GZ_F32) return ((const float*)g)[i];
-  if (dtype == GZ_F16) return __half2float(((const __half*)g)[i]);
-  return __bfloat162float(((const __nv_bfloat16*)g)[i]);
+// A lane's eight elements of a 256-element block: four from 4 lane on and four
+// from 128 + 4 lane on, so that every access of a warp is one run of memory.
+constexpr int kRun = 4;
+__device__ __forceinline__ int place(int lane, int k) { return (k / kRun) * (kBlock / 2) + lane * kRun + k % kRun; }
+
+// Vector accesses of a lane's elements i, i + 1, .. i + 3.
+__device__ __forceinline__ void load4(float* x, const float* p) { *(float4*)x = __ldcs((const float4*)p); }
+__device__ __forceinline__ void load4(float* x, const __half* p) {
+  const uint2 raw = __ldcs((const uint2*)p);
+  const float2 a = __half22float2(*(const __half2*)&raw.x), b = __half22float2(*(const __half2*)&raw.y);
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+__device__ __forceinline__ void load4(float* x, const __nv_bfloat16* p) {
+  const uint2 raw = __ldcs((const uint2*)p);
+  x[0] = __uint_as_float(raw.x << 16), x[1] = __uint_as_float(raw.x & 0xffff0000u);
+  x[2] = __uint_as_float(raw.y << 16), x[3] = __uint_as_float(raw.y & 0xffff0000u);
 }
 
+// Gradients of a lane, zeros beyond the tensor's end.  `vector`: a whole block
+// whose gradients are aligned to four of them.
+__device__ __forceinline__ void load_grads(float* x, const void* g, int dtype, int64_t at, int lane, int64_t n, bool vector) {
+#pragma unroll
+  for (int k = 0; k < kPerLane; k += kRun) {
+    const int64_t i = at + place(lane, k);
+    if (vector) {
+      if (dtype == GZ_F32) load4(x + k, (const float*)g + i);
+      else if (dtype == GZ_F16) load4(x + k, (const __half*)g + i);
+      else load4(x + k, (const __nv_bfloat16*)g + i);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kRun; ++q) {
+        x[k + q] = 0.f;
+        if (i + q >= n) continue;
+        if (dtype == GZ_F32) x[k + q] = ((const float*)g)[i + q];
+        else if (dtype == GZ_F16) x[k + q] = __half2float(((const __half*)g)[i + q]);
+        else x[k + q] = __bfloat162float(((const __nv_bfloat16*)g)[i + q]);
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool grads_aligned(const void* g, int dtype) {
+  return ((uintptr_t)g & (dtype == GZ_F32 ? 15 : 7)) == 0;
+}
+
+// Sum of squares: eight products added in pairs in 32 bits, everything above
+// them in 64.  One block's last arrival adds the chunks' sums, in their order.
 __global__ void __launch_bounds__(kThreads) norm_kernel(StepArgs a, const __grid_constant__ Grads grads) {
   __shared__ double sums[kThreads / 32];
   __shared__ bool last;
   const Chunk c = a.chunks[blockIdx.x];
-  const Tensor& t = a.tensors[c.tensor];
+  const int64_t n = a.tensors[c.tensor].n;
   const void* g = grads.p[c.tensor - a.first_tensor];
   const int dtype = grads.dtype[c.tensor - a.first_tensor];
-  const int64_t begin = (int64_t)c.block * kBlock;
-  const int64_t end = min(t.n, begin + (int64_t)a.blocks * kBlock);
+  const int lane = threadIdx.x % 32;
+  const bool aligned = grads_aligned(g, dtype);
   double sum = 0;
   if (g)
-    for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) {
-      const float x = load_grad(g, dtype, i);
-      sum += (double)x * x;
+#pragma unroll 2
+    for (uint32_t b = threadIdx.x / 32; b < a.blocks; b += kThreads / 32) {
+      const int64_t at = (int64_t)(c.block + b) * kBlock;
+      if (at >= n) break;
+      float x[kPerLane];
+      load_grads(x, g, dtype, at, lane, n, aligned && at + kBlock <= n);
+#pragma unroll
+      for (int k = 0; k < kPerLane; ++k) x[k] *= x[k];
+      sum += (double)(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
     }
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+  if (lane == 0) sums[threadIdx.x / 32] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0;
@@ -104,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(StepArgs a, const __grid
   sum = 0;
   for (int i = threadIdx.x; i < a.chunk_count; i += kThreads) sum += __ldcg(&a.partial[i]);
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+  if (lane == 0) sums[threadIdx.x / 32] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0;
@@ -123,88 +169,277 @@ __device__ __forceinline__ int scale_exponent(float most) {
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// x (already scaled) as an 8-bit float, rounded down or up by u in [0, 1).
-__device__ __forceinline__ uint8_t to_8bit(float x, float u, bool nonzero) {
-  const float y = fabsf(x);
-  const int e = max((int)(__float_as_uint(y) >> 23) - 127, -6);
-  float q = floorf(__fadd_rn(__fmul_rn(y, power(3 - e)), u));
-  if (nonzero && q == 0.f && y > 0.f) q = 1.f;
-  q = copysignf(__fmul_rn(q, power(e - 3)), x);
-  return (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+// x (already scaled, finite) rounded down or up by u = h 2^-16 to a value of the
+// 8-bit format: a multiple of a grain of 2^(e - 3), e the exponent, at least -6.
+// From 2^-6 on that is the float's upper 12 bits after adding u of a grain to
+// its bits; below, the sum is taken in 32 bits.
+__device__ __forceinline__ float to_8bit(float x, uint32_t h) {
+  return __uint_as_float((__float_as_uint(x) + (h << 4)) & 0xfff00000u);
+}
+constexpr float kSmall = 0x1p-6f;
+template <bool kRoot> __device__ __forceinline__ float small_to_8bit(float x, uint32_t h) {
+  float q = floorf(__fadd_rn(fabsf(x) * 512.f, (float)h * 0x1p-16f));
+  if (kRoot && q == 0.f && x > 0.f) q = 1.f;  // a root stays positive: m over it must not run away
+  return copysignf(q * 0x1p-9f, x);
+}
+// Four such values' codes, and back.
+__device__ __forceinline__ uint32_t codes(const float* q) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+__device__ __forceinline__ void values(float* x, uint32_t c) {
+#pragma unroll
+  for (int k = 0; k < 4; k += 2) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> (8 * k)), __NV_E4M3);
+    const float2 f = __half22float2(*(const __half2*)&h);
+    x[k] = f.x;
+    x[k + 1] = f.y;
+  }
 }
 
-__device__ __forceinline__ float from_8bit(uint8_t q) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3)));
+// Largest magnitude over the warp (as bits: they order like the values).
+__device__ __forceinline__ float warp_most(const float* x) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) most = max(most, __float_as_uint(x[k]) & 0x7fffffffu);
+  most = __reduce_max_sync(~0u, most);
+  if (most >= 0x7f800000u) {  // of the finite ones
+    most = 0;
+#pragma unroll
+    for (int k = 0; k < kPerLane; ++k) {
+      const uint32_t b = __float_as_uint(x[k]) & 0x7fffffffu;
+      if (b < 0x7f800000u) most = max(most, b);
+    }
+    most = __reduce_max_sync(~0u, most) | 0x80000000u;  // the sign tells
+  }
+  return __uint_as_float(most);
 }
 
-__device__ __forceinline__ float warp_max(float x) {
-  for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
-  return x;
-}
+// What a lane reads of a whole, aligned block.
+template <int kBits> struct Raw {
+  float4 p[2];
+  uint4 g[2];  // as read: four floats, or four 16-bit numbers in x and y
+  float4 m[kBits == 32 ? 2 : 1], v[kBits == 32 ? 2 : 1];
+  uint32_t mc[2], vc[2];
+  float ms, vs;
 
-// A warp per 256-element block, eight neighbouring elements per lane.
+  __device__ __forceinline__ void load(const Tensor& t, const void* grad, int dtype, uint32_t block, int lane) {
+    const int64_t at = (int64_t)block * kBlock;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t i = at + place(lane, k * kRun);
+      p[k] = __ldcs((const float4*)(t.param + i));
+      if (dtype == GZ_F32) {
+        g[k] = __ldcs((const uint4*)((const float*)grad + i));
+      } else {
+        const uint2 h = __ldcs((const uint2*)((const uint16_t*)grad + i));
+        g[k] = make_uint4(h.x, h.y, 0, 0);
+      }
+      if (kBits == 32) {
+        m[k] = __ldcs((const float4*)((const float*)t.m + i));
+        v[k] = __ldcs((const float4*)((const float*)t.v + i));
+      } else {
+        mc[k] = __ldcs((const uint32_t*)((const uint8_t*)t.m + i));
+        vc[k] = __ldcs((const uint32_t*)((const uint8_t*)t.v + i));
+      }
+    }
+    if (kBits == 8) {
+      ms = t.m_scale[block];
+      vs = t.v_scale[block];
+    }
+  }
+  __device__ __forceinline__ void grads(float* x, int dtype) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float* y = x + k * kRun;
+      if (dtype == GZ_F32) {
+        *(uint4*)y = g[k];
+      } else if (dtype == GZ_F16) {
+        *(float2*)y = __half22float2(*(const __half2*)&g[k].x);
+        *(float2*)(y + 2) = __half22float2(*(const __half2*)&g[k].y);
+      } else {
+        y[0] = __uint_as_float(g[k].x << 16), y[1] = __uint_as_float(g[k].x & 0xffff0000u);
+        y[2] = __uint_as_float(g[k].y << 16), y[3] = __uint_as_float(g[k].y & 0xffff0000u);
+      }
+    }
+  }
+};
+
+// The numbers of a step that a chunk's tensor goes by.
+struct Rates {
+  float decay, step, scale;
+  __device__ Rates(const StepArgs& a, const Tensor& t) {
+    decay = (float)(1.0 - a.lr * t.lr_scale * t.weight_decay);
+    step = (float)(a.lr_corrected * t.lr_scale);
+    scale = a.grad_scale;
+    if (a.max_norm > 0.f) scale = __fmul_rn(scale, fminf(__fdiv_rn(a.max_norm, __fadd_rn(*a.norm, 1e-6f)), 1.f));
+  }
+};
+
+// The update of a lane's elements; v holds the root of the second moment going
+// in with 8-bit states, and root the new one's.
 template <int kBits>
-__global__ void __launch_bounds__(kThreads) step_kernel(StepArgs a, const __grid_constant__ Grads grads) {
+__device__ __forceinline__ void update(const StepArgs& a, const Rates& rate, float* x, float* p, float* m, float* v, float* root) {
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    if (kBits == 8) v[k] = __fmul_rn(v[k], v[k]);
+    x[k] = __fmul_rn(x[k], rate.scale);
+    m[k] = __fadd_rn(__fmul_rn(m[k], a.beta1), __fmul_rn(x[k], a.one_beta1));
+    v[k] = __fadd_rn(__fmul_rn(v[k], a.beta2), __fmul_rn(__fmul_rn(x[k], x[k]), a.one_beta2));
+    root[k] = __fsqrt_rn(v[k]);
+    const float move = __fdiv_rn(m[k], __fadd_rn(__fmul_rn(root[k], a.correct2), a.eps));
+    p[k] = __fsub_rn(__fmul_rn(p[k], rate.decay), __fmul_rn(move, rate.step));
+  }
+}
+
+// Rounds a block's new states to 8 bits and stores them.
+__device__ __forceinline__ void store_8bit(const StepArgs& a, const Tensor& t, uint32_t block, int lane, float* m, float* root) {
+  const int64_t at = (int64_t)block * kBlock;
+  const float m_most = warp_most(m), v_most = warp_most(root);
+  const int me = scale_exponent(fabsf(m_most)), ve = scale_exponent(fabsf(v_most));
+  const float m_down = power(-me), v_down = power(-ve);
+  const bool odd = signbit(m_most) || signbit(v_most);  // something is not finite
+  const uint32_t first = (uint32_t)(t.first + at) + lane * kRun + a.key;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    const uint32_t h = mix32(first + place(0, k));
+    const float x = __fmul_rn(m[k], m_down), y = __fmul_rn(root[k], v_down);
+    m[k] = to_8bit(x, h & 0xffffu);
+    root[k] = to_8bit(y, h >> 16);
+    if (fabsf(x) < kSmall || y < kSmall) {
+      if (fabsf(x) < kSmall) m[k] = small_to_8bit<false>(x, h & 0xffffu);
+      if (y < kSmall) root[k] = small_to_8bit<true>(y, h >> 16);
+    }
+    if (odd) {
+      if (!isfinite(x)) m[k] = NAN;
+      if (!isfinite(y)) root[k] = NAN;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPerLane; k += kRun) {
+    __stcs((uint32_t*)((uint8_t*)t.m + at + place(lane, k)), codes(m + k));
+    __stcs((uint32_t*)((uint8_t*)t.v + at + place(lane, k)), codes(root + k));
+  }
+  if (lane == 0) {
+    t.m_scale[block] = power(me);
+    t.v_scale[block] = power(ve);
+  }
+}
+
+// A block at a tensor's end, or of one that is not aligned: element by element.
+template <int kBits>
+__device__ __noinline__ void step_ragged(const StepArgs& a, const Tensor* tensor, const void* g, int dtype, uint32_t block, int lane) {
+  const Tensor t = *tensor;
+  const Rates rate(a, t);
+  const int64_t at = (int64_t)block * kBlock;
+  float x[kPerLane], p[kPerLane], m[kPerLane], v[kPerLane], root[kPerLane];
+  const float ms = kBits == 8 ? t.m_scale[block] : 1.f, vs = kBits == 8 ? t.v_scale[block] : 1.f;
+#pragma unroll
+  for (int k = 0; k < kPerLane; k += kRun) {
+    if (kBits == 8) {  // states are whole blocks
+      values(m + k, *(const uint32_t*)((const uint8_t*)t.m + at + place(lane, k)));
+      values(v + k, *(const uint32_t*)((const uint8_t*)t.v + at + place(lane, k)));
+    }
+  }
+  load_grads(x, g, dtype, at, lane, t.n, false);
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    const int64_t i = at + place(lane, k);
+    const bool in = i < t.n;
+    p[k] = in ? t.param[i] : 0.f;
+    if (kBits == 32) {
+      m[k] = in ? ((const float*)t.m)[i] : 0.f;
+      v[k] = in ? ((const float*)t.v)[i] : 0.f;
+    } else {
+      m[k] = in ? __fmul_rn(m[k], ms) : 0.f;
+      v[k] = in ? __fmul_rn(v[k], vs) : 0.f;
+    }
+  }
+  update<kBits>(a, rate, x, p, m, v, root);
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    const int64_t i = at + place(lane, k);
+    if (i >= t.n) continue;
+    t.param[i] = p[k];
+    if (kBits == 32) {
+      ((float*)t.m)[i] = m[k];
+      ((float*)t.v)[i] = v[k];
+    }
+    if (t.copy) {
+      if (t.copy_dtype == GZ_F16) ((__half*)t.copy)[i] = __float2half_rn(p[k]);
+      else ((__nv_bfloat16*)t.copy)[i] = __float2bfloat16_rn(p[k]);
+    }
+  }
+  if (kBits == 8) store_8bit(a, t, block, lane, m, root);
+}
+
+// A warp per 256-element block, several in turn; with 8-bit states the next
+// block is read while one is worked on.  Every array is read and written once,
+// past the caches (nothing is used again within the step): bound by memory.
+template <int kBits>
+__global__ void __launch_bounds__(kThreads, kStepBlocks) step_kernel(const __grid_constant__ StepArgs a, const __grid_constant__ Grads grads) {
   const Chunk c = a.chunks[blockIdx.x];
   const Tensor t = a.tensors[c.tensor];
   const void* g = grads.p[c.tensor - a.first_tensor];
   const int dtype = grads.dtype[c.tensor - a.first_tensor];
   if (!g) return;
   const int lane = threadIdx.x % 32;
-  const float decay = (float)(1.0 - a.lr * t.lr_scale * t.weight_decay);
-  const float step = (float)(a.lr_corrected * t.lr_scale);
-  float scale = a.grad_scale;
-  if (a.max_norm > 0.f) scale = __fmul_rn(scale, fminf(__fdiv_rn(a.max_norm, __fadd_rn(*a.norm, 1e-6f)), 1.f));
-  const uint32_t blocks = (uint32_t)((t.n + kBlock - 1) / kBlock);
-  const uint32_t end = min(blocks, c.block + a.blocks);
-  for (uint32_t b = c.block + threadIdx.x / 32; b < end; b += kThreads / 32) {
-    const int64_t at = (int64_t)b * kBlock + lane * kPerLane;
-    float m[kPerLane], v[kPerLane], root[kPerLane];
-    const float ms = kBits == 8 ? t.m_scale[b] : 1.f, vs = kBits == 8 ? t.v_scale[b] : 1.f;
-    float m_most = 0.f, v_most = 0.f;
-    for (int k = 0; k < kPerLane; ++k) {
-      const int64_t i = at + k;
-      m[k] = v[k] = root[k] = 0.f;
-      if (i >= t.n) continue;
-      const float x = __fmul_rn(load_grad(g, dtype, i), scale);
-      if (kBits == 8) {
-        m[k] = __fmul_rn(from_8bit(((const uint8_t*)t.m)[i]), ms);
-        const float r = __fmul_rn(from_8bit(((const uint8_t*)t.v)[i]), vs);
-        v[k] = __fmul_rn(r, r);
-      } else {
-        m[k] = ((const float*)t.m)[i];
-        v[k] = ((const float*)t.v)[i];
-      }
-      m[k] = __fadd_rn(__fmul_rn(m[k], a.beta1), __fmul_rn(x, a.one_beta1));
-      v[k] = __fadd_rn(__fmul_rn(v[k], a.beta2), __fmul_rn(__fmul_rn(x, x), a.one_beta2));
-      root[k] = __fsqrt_rn(v[k]);
-      const float move = __fdiv_rn(m[k], __fadd_rn(__fmul_rn(root[k], a.correct2), a.eps));
-      const float p = __fsub_rn(__fmul_rn(t.param[i], decay), __fmul_rn(move, step));
-      t.param[i] = p;
-      if (t.copy) {
-        if (t.copy_dtype == GZ_F16) ((__half*)t.copy)[i] = __float2half_rn(p);
-        else ((__nv_bfloat16*)t.copy)[i] = __float2bfloat16_rn(p);
-      }
+  const Rates rate(a, t);
+  bool aligned = grads_aligned(g, dtype) && ((uintptr_t)t.param & 15) == 0 && ((uintptr_t)t.copy & 7) == 0;
+  if (kBits == 32) aligned = aligned && (((uintptr_t)t.m | (uintptr_t)t.v) & 15) == 0;
+  const uint32_t end = min((uint32_t)((t.n + kBlock - 1) / kBlock), c.block + a.blocks);
+  const uint32_t whole = aligned ? min((uint32_t)(t.n / kBlock), end) : 0;  // whole blocks end here
+  uint32_t b = c.block + threadIdx.x / 32;
+  Raw<kBits> next;
+  if (b < whole) next.load(t, g, dtype, b, lane);
+#pragma unroll 2
+  for (; b < whole; b += kThreads / 32) {
+    const Raw<kBits> now = next;
+    if (kBits == 8 && b + kThreads / 32 < whole) next.load(t, g, dtype, b + kThreads / 32, lane);
+    float x[kPerLane], p[kPerLane], m[kPerLane], v[kPerLane], root[kPerLane];
+    now.grads(x, dtype);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      *(float4*)(p + k * kRun) = now.p[k];
       if (kBits == 32) {
-        ((float*)t.m)[i] = m[k];
-        ((float*)t.v)[i] = v[k];
-      }
-      if (isfinite(m[k])) m_most = fmaxf(m_most, fabsf(m[k]));
-      if (isfinite(root[k])) v_most = fmaxf(v_most, root[k]);
-    }
-    if (kBits == 8) {
-      const int me = scale_exponent(warp_max(m_most)), ve = scale_exponent(warp_max(v_most));
-      for (int k = 0; k < kPerLane; ++k) {
-        const uint32_t h = mix32((uint32_t)(t.first + at + k) + a.key);
-        ((uint8_t*)t.m)[at + k] = to_8bit(__fmul_rn(m[k], power(-me)), (float)(h & 0xffffu) * 0x1p-16f, false);
-        ((uint8_t*)t.v)[at + k] = to_8bit(__fmul_rn(root[k], power(-ve)), (float)(h >> 16) * 0x1p-16f, true);
-      }
-      if (lane == 0) {
-        t.m_scale[b] = power(me);
-        t.v_scale[b] = power(ve);
+        *(float4*)(m + k * kRun) = now.m[k];
+        *(float4*)(v + k * kRun) = now.v[k];
+      } else {
+        values(m + k * kRun, now.mc[k]);
+        values(v + k * kRun, now.vc[k]);
+#pragma unroll
+        for (int q = k * kRun; q < (k + 1) * kRun; ++q) {
+          m[q] = __fmul_rn(m[q], now.ms);
+          v[q] = __fmul_rn(v[q], now.vs);
+        }
       }
     }
+    update<kBits>(a, rate, x, p, m, v, root);
+#pragma unroll
+    for (int k = 0; k < kPerLane; k += kRun) {
+      const int64_t i = (int64_t)b * kBlock + place(lane, k);
+      __stcs((float4*)(t.param + i), *(const float4*)(p + k));
+      if (kBits == 32) {
+        __stcs((float4*)((float*)t.m + i), *(const float4*)(m + k));
+        __stcs((float4*)((float*)t.v + i), *(const float4*)(v + k));
+      }
+      if (t.copy) {
+        uint2 raw;
+        if (t.copy_dtype == GZ_F16) {
+          ((__half2*)&raw)[0] = __floats2half2_rn(p[k], p[k + 1]);
+          ((__half2*)&raw)[1] = __floats2half2_rn(p[k + 2], p[k + 3]);
+        } else {
+          ((__nv_bfloat162*)&raw)[0] = __floats2bfloat162_rn(p[k], p[k + 1]);
+          ((__nv_bfloat162*)&raw)[1] = __floats2bfloat162_rn(p[k + 2], p[k + 3]);
+        }
+        __stcs((uint2*)((uint16_t*)t.copy + i), raw);
+      }
+    }
+    if (kBits == 8) store_8bit(a, t, b, lane, m, root);
+    else if (b + kThreads / 32 < whole) next.load(t, g, dtype, b + kThreads / 32, lane);
   }
+  for (; b < end; b += kThreads / 32) step_ragged<kBits>(a, a.tensors + c.tensor, g, dtype, b, lane);
 }
 
 }  // namespace
@@ -269,7 +504,11 @@ gz_status create(const gz_adamw_tensor* tensors, int count, int state_bits, int 
   a->device = device;
   a->state_bits = state_bits;
   a->count = count;
+  // a block of the plan's units per warp and round; with many, more rounds
+  // until there are some sixteen chunks an SM
+  const uint64_t all_blocks = first / kBlock;
   a->blocks_per_chunk = 8;
+  while (a->blocks_per_chunk < 64 && all_blocks / a->blocks_per_chunk > 148 * 32) a->blocks_per_chunk *= 2;
   for (int k = 0; k < count; ++k) {
     a->chunk_start.push_back((int)chunks.size());
     const uint64_t blocks = (uint64_t)(table[k].n + kBlock - 1) / kBlock;
