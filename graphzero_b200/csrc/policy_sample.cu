@@ -35,11 +35,13 @@ struct SampleArgs {
   int32_t* action;
   float* logp;
   int64_t first_row, end_row;  // of this launch
+  int row_warps;               // warps a masked row gets
 };
 
 constexpr int kList = 2048;         // keys a block's list holds
 constexpr int kWarpRow = 256;       // actions of a row that a warp takes
 constexpr int kBins = 1024;         // of the histogram, which the list's memory holds
+constexpr int kMaskedList = 1024, kMaskedThreads = 128;  // the same for masked rows, and their blocks
 constexpr int kSampleThreads = 512;  // most threads of a block
 constexpr int64_t kRowsPerLaunch = 1 << 28;
 
@@ -119,27 +121,45 @@ template <typename T> struct Row {
   __device__ uint4 vector(int v) const { return __ldg((const uint4*)(x + head) + v); }
 };
 
+// f(first, bits) for this thread's share of a mask, sixteen bytes at a time and
+// the bytes beside the whole sixteens one by one: bits of visible actions from
+// `first` on, none of them 0.  Needs at least 30 threads.
+template <int kAhead, typename T, typename F> __device__ __forceinline__ void each_visible(const Row<T>& r, int tid, int n, F f) {
+  const int head = min(r.actions, (int)(-(uintptr_t)r.mask & 15));
+  const int groups = (r.actions - head) / 16, ends = r.actions - groups * 16;
+  const int ej = tid < head ? tid : r.actions - ends + tid;
+  if (tid < ends && r.mask[ej]) f(ej, 1u);
+  const uint4* group = (const uint4*)(r.mask + head);
+  for (int u0 = tid; u0 < groups; u0 += kAhead * n) {
+    uint4 w[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) w[i] = u0 + i * n < groups ? __ldg(group + u0 + i * n) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (!(w[i].x | w[i].y | w[i].z | w[i].w)) continue;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // the bytes' flags, gathered into four bits
+        const uint32_t c = __vcmpne4(k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w, 0) & 0x08040201u;
+        bits |= (c * 0x01010101u >> 24) << (4 * k);
+      }
+      f(head + (u0 + i * n) * 16, bits);
+    }
+  }
+}
+
 // f(j, score) for this thread's share of the visible actions.
 template <typename T, typename F> __device__ __forceinline__ void each(const Row<T>& r, int tid, int n, F f) {
   auto one = [&](int j, float v) {
     if (v > -INFINITY) f(j, fminf(v, FLT_MAX));  // a NaN counts as -inf
   };
   if (r.mask) {
-    const int head = min(r.actions, (int)(-(uintptr_t)r.mask & 15));
-    const int groups = (r.actions - head) / 16, ends = r.actions - groups * 16;
-    const int ej = tid < head ? tid : r.actions - ends + tid;
-    if (tid < ends && r.mask[ej]) one(ej, to_f32(r.x[ej]));
-#pragma unroll 2
-    for (int u = tid; u < groups; u += n) {
-      const uint4 w = __ldg((const uint4*)(r.mask + head) + u);
-      if (!(w.x | w.y | w.z | w.w)) continue;
-#pragma unroll 1
-      for (int k = 0; k < 4; ++k)
-        for (uint32_t bits = __vcmpne4(k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w, 0) & 0x01010101u; bits; bits &= bits - 1) {
-          const int j = head + u * 16 + k * 4 + (__ffs(bits) - 1) / 8;
-          one(j, to_f32(r.x[j]));
-        }
-    }
+    each_visible<2>(r, tid, n, [&](int first, uint32_t bits) {
+      for (; bits; bits &= bits - 1) {
+        const int j = first + __ffs(bits) - 1;
+        one(j, to_f32(r.x[j]));
+      }
+    });
   } else {
     if (tid < r.ends) one(r.end_index(tid), to_f32(r.x[r.end_index(tid)]));
     for (int v = tid; v < r.vecs; v += n) {
@@ -257,32 +277,140 @@ __device__ bool draw_from_list(const SampleArgs& a, int64_t row, const Team<kWar
   return true;
 }
 
+// Draws from at most kFew actions, in any order, with one warp: every key's rank
+// and the weight before it come from comparing it with all others.  A lane
+// brings kMine of them, j < 0 for none.  row_weight and the answer as in
+// draw_from_list.
+constexpr int kFew = 64, kMine = kFew / 32;
+struct FewShared {
+  uint64_t key[kFew], weight[kFew];
+};
+template <typename T>
+__device__ __forceinline__ bool draw_from_few(const SampleArgs& a, int64_t row, const Row<T>& r, const Filters& f, const int* j,
+                                              const float* x, double row_weight, FewShared& sh) {
+  const Team<true> team{nullptr, (int)threadIdx.x % 32, 32};
+  float noise[kMine], d[kMine], e[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) noise[i] = r.noise && j[i] >= 0 ? r.noise[j[i]] : 0.f;
+  uint64_t key[kMine], best = 0;
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const bool in = j[i] >= 0 && x[i] > -INFINITY;  // a NaN counts as -inf
+    key[i] = in ? rank_key(fminf(x[i], FLT_MAX), j[i]) : 0;
+    if (key[i] > best) best = key[i];
+    count += __popc(__ballot_sync(~0u, in));
+  }
+  best = team.max(best);
+  if (!best || f.greedy) {
+    if (team.tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
+    return true;
+  }
+  const float top = key_score(best);
+  uint64_t weight[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    d[i] = f.depth(key_score(key[i]), top);
+    e[i] = key[i] ? expf(d[i]) : 0.f;
+    weight[i] = fixed_weight(e[i]);
+  }
+  bool keep[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) keep[i] = key[i] != 0;
+  if ((f.top_k > 0 && f.top_k < count) || f.top_p < 1.f) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      sh.key[team.tid + 32 * i] = key[i];
+      sh.weight[team.tid + 32 * i] = weight[i];
+    }
+    team.sync();
+    int rank[kMine] = {};
+    uint64_t before[kMine] = {}, sum = 0;
+    const int most = 32 - __clz(__ballot_sync(~0u, j[kMine - 1] >= 0)), full = most ? 32 * (kMine - 1) + most : 32;
+    for (int q = 0; q < full; ++q) {
+      const uint64_t k = sh.key[q], w = sh.weight[q];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (k > key[i]) {
+          ++rank[i];
+          before[i] += w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      if (f.top_k > 0) keep[i] = keep[i] && rank[i] < f.top_k;
+      if (keep[i]) sum += weight[i];
+    }
+    if (f.top_p < 1.f) {
+      const double total = (double)team.sum(sum), goal = f.top_p * (row_weight < 0 ? total : row_weight);
+      if (total < goal) return false;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) keep[i] = keep[i] && ((double)before[i] < goal || rank[i] == 0);
+    }
+  }
+  uint64_t sum = 0;
+  best = 0;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+    if (keep[i] && e[i] >= f.min_p) {
+      sum += weight[i];
+      const float s = d[i] + noise[i];
+      const uint64_t k = rank_key(s >= -INFINITY ? s : -INFINITY, key_index(key[i]));
+      if (k > best) best = k;
+    }
+  sum = team.sum(sum);
+  best = team.max(best);
+  // the drawn action's lane answers
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+    if (key[i] && key_index(key[i]) == key_index(best)) answer(a, row, key_index(best), d[i] - logf((float)((double)sum * 0x1p-44)));
+  return true;
+}
+
 // Rows of at most kWarpRow actions: a warp each, four a block.
 template <typename T> __global__ void __launch_bounds__(128) sample_warp_kernel(SampleArgs a) {
   __shared__ uint64_t lists[4][kWarpRow];
+  __shared__ FewShared few[4];
   const int64_t row = a.first_row + (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= a.end_row) return;
   const Team<true> team{nullptr, (int)threadIdx.x % 32, 32};
   const Row<T> r(a, row);
   const Filters f(a.cfg, row);
+  auto score = [&](int j) { return j < r.actions && !(r.mask && !r.mask[j]) ? to_f32(r.x[j]) : -INFINITY; };
+  if (r.actions <= kFew) {
+    int j[kMine];
+    float x[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      j[i] = team.tid + 32 * i < r.actions ? team.tid + 32 * i : -1;
+      x[i] = j[i] >= 0 ? score(j[i]) : -INFINITY;
+    }
+    draw_from_few(a, row, r, f, j, x, -1.0, few[threadIdx.x / 32]);
+    return;
+  }
   uint64_t* keys = lists[threadIdx.x / 32];
   uint64_t best = 0;
   int count = 0;
-  for (int j = team.tid; j < r.actions; j += 32) {
-    const float v = r.mask && !r.mask[j] ? -INFINITY : to_f32(r.x[j]);
-    const uint64_t key = v > -INFINITY ? rank_key(fminf(v, FLT_MAX), j) : 0;
-    keys[j] = key;
-    count += key != 0;
-    if (key > best) best = key;
+#pragma unroll 2
+  for (int j0 = 0; j0 < r.actions; j0 += 32) {
+    const int j = j0 + team.tid;
+    const float v = score(j);
+    const bool in = v > -INFINITY;
+    const uint32_t all = __ballot_sync(~0u, in);
+    if (in) {
+      const uint64_t key = rank_key(fminf(v, FLT_MAX), j);
+      keys[count + __popc(all & ((1u << team.tid) - 1))] = key;
+      if (key > best) best = key;
+    }
+    count += __popc(all);
   }
   best = team.max(best);
-  count = team.sum(count);
   team.sync();
   if (!best || f.greedy) {
     if (team.tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
     return;
   }
-  draw_from_list(a, row, team, r, f, keys, r.actions, count, key_score(best), -1.0);
+  draw_from_list(a, row, team, r, f, keys, count, count, key_score(best), -1.0);
 }
 
 // The rank key of the last kept action: the largest with at least `goal` (a
@@ -303,7 +431,7 @@ __device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, cons
 
 // The same through a histogram of kBins bins over the 31 temperatures below the
 // best score (what lies deeper, by bisection if need be).
-template <bool kWeights, typename T>
+template <bool kWeights, int kSize, typename T>
 __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal,
                                               uint64_t* memory, int* counter) {
   __shared__ uint64_t above;
@@ -340,12 +468,12 @@ __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row
   each(r, team.tid, team.n, [&](int j, float x) {
     if (bin(x) == b) {
       const int at = atomicAdd(counter, 1);
-      if (at < kList) memory[at] = rank_key(x, j);
+      if (at < kSize) memory[at] = rank_key(x, j);
     }
   });
   team.sync();
   const int m = *counter;
-  if (m > kList) return last_by_bisection<kWeights>(team, r, f, top, goal);
+  if (m > kSize) return last_by_bisection<kWeights>(team, r, f, top, goal);
   sort_keys(team, memory, m);
   const int kept = keys_before<kWeights>(team, memory, m, f, top, goal, base, nullptr);
   const uint64_t last = memory[max(0, kept - 1)];
@@ -353,16 +481,15 @@ __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row
   return last;
 }
 
-struct Shared {
-  uint64_t slots[kSampleThreads / 32], list[kList];
+template <int kSize> struct Shared {
+  uint64_t slots[kSampleThreads / 32], list[kSize];
   int counter;
 };
 
 // A row whose visible actions do not all fit the list.
-template <typename T, bool kMasked>
-__device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
+template <typename T, bool kMasked, int kSize>
+__device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh) {
   constexpr int V = Row<T>::V;
-  const int64_t row = a.first_row + blockIdx.x;
   const int tid = threadIdx.x, n = blockDim.x;
   const Team<false> team{sh.slots, tid, n};
   const Row<T> r(a, row);
@@ -454,15 +581,45 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
       }
       row_weight = (double)team.sum(z) * 0x1p44;
     }
-    const int rank = by_count ? f.top_k : n / 2;
-    if (rank <= n) {
-      // the largest number, to 20 bits, that `rank` threads' best scores reach
-      uint32_t reach = 0;
+    // The largest number that enough threads' best scores reach: top_k of them;
+    // or so many that they weigh top_p of the row, or else half of them, which
+    // with what lies between them may still be enough.  One warp searches for
+    // it, over the scores' upper 20 bits, with weights in units of 2^-22.
+    if (!by_count || f.top_k <= n) {
+      uint32_t* scores = (uint32_t*)sh.list;
+      scores[tid] = (uint32_t)(mine >> 18);
+      __syncthreads();
+      if (tid < 32) {
+        uint32_t score[kSampleThreads / 32], weight[kSampleThreads / 32];
+#pragma unroll
+        for (int i = 0; i < kSampleThreads / 32; ++i) {
+          score[i] = i < n / 32 ? scores[tid + 32 * i] : 0;
+          weight[i] = by_count ? 1 : score[i] ? (uint32_t)(expf(f.depth(key_value(score[i]), top)) * 0x1p22f) : 0;
+        }
+        auto above = [&](uint32_t mid) {
+          uint32_t c = 0;
+#pragma unroll
+          for (int i = 0; i < kSampleThreads / 32; ++i) c += score[i] >= mid ? weight[i] : 0;
+          return __reduce_add_sync(~0u, c);
+        };
+        uint32_t goal = f.top_k;
+        if (!by_count) {
+          const double g = f.top_p * row_weight * 0x1p-22 * 1.00001 + 1;
+          goal = g < 0x1p31 ? (uint32_t)g : ~0u;
+          if (above(1) < goal) {
+            goal = n / 2;
+#pragma unroll
+            for (int i = 0; i < kSampleThreads / 32; ++i) weight[i] = 1;
+          }
+        }
+        uint32_t most = 0;
 #pragma unroll 1
-      for (int bit = 31; bit >= 12; --bit) {
-        const uint32_t mid = reach | 1u << bit;
-        if (__syncthreads_count((uint32_t)(mine >> 18) >= mid) >= rank) reach = mid;
+        for (int bit = 31; bit >= 12; --bit)
+          if (above(most | 1u << bit) >= goal) most |= 1u << bit;
+        if (tid == 0) *(uint32_t*)sh.slots = most;
       }
+      __syncthreads();
+      const uint32_t reach = *(uint32_t*)sh.slots;
       if (reach) {
         const float from = key_value(reach);
         if (tid == 0) sh.counter = 0;
@@ -470,7 +627,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
         auto take = [&](int j, float x) {
           if (x >= from) {
             const int at = atomicAdd(&sh.counter, 1);
-            if (at < kList) sh.list[at] = rank_key(x, j);
+            if (at < kSize) sh.list[at] = rank_key(x, j);
           }
         };
         if (kMasked) {
@@ -490,10 +647,25 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
         }
         __syncthreads();
         const int m = sh.counter;
-        if (m <= kList && draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
+        if (m <= kFew) {
+          if (tid < 32) {
+            int j[kMine];
+            float x[kMine];
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              const uint64_t key = tid + 32 * i < m ? sh.list[tid + 32 * i] : 0;
+              j[i] = key ? key_index(key) : -1;
+              x[i] = key_score(key);
+            }
+            const bool done = draw_from_few(a, row, r, f, j, x, row_weight, *(FewShared*)(sh.list + kFew));
+            if (tid == 0) sh.counter = done;
+          }
+          __syncthreads();
+          if (sh.counter) return;
+        } else if (m <= kSize && draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
       }
     }
-    if (by_count) last = last_by_bins<false>(team, r, f, top, (double)f.top_k, sh.list, &sh.counter);
+    if (by_count) last = last_by_bins<false, kSize>(team, r, f, top, (double)f.top_k, sh.list, &sh.counter);
     if (by_weight) {
       if (by_count) {
         uint64_t w = 0;
@@ -502,7 +674,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
         });
         row_weight = (double)team.sum(w);
       }
-      const uint64_t cut = last_by_bins<true>(team, r, f, top, f.top_p * row_weight, sh.list, &sh.counter);
+      const uint64_t cut = last_by_bins<true, kSize>(team, r, f, top, f.top_p * row_weight, sh.list, &sh.counter);
       if (cut > last) last = cut;
     }
   }
@@ -514,37 +686,101 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, Shared& sh) {
 }
 
 // A call of its own, so that rows that fit the list do not pay for its registers.
-template <typename T, bool kMasked> __device__ __noinline__ void draw_long_call(const SampleArgs& a, Shared& sh) {
-  draw_long<T, kMasked>(a, sh);
+template <typename T, int kSize> __device__ __noinline__ void draw_masked_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh) {
+  draw_long<T, true>(a, row, sh);
 }
 
-// Rows that are expected to fit the list: masked, or of at most kList actions.
-template <typename T, bool kMasked>
-__global__ void __launch_bounds__(kSampleThreads, 4) sample_list_kernel(const __grid_constant__ SampleArgs a) {
-  __shared__ Shared sh;
+// Masked rows, in blocks of `row_warps` warps for every row: the mask gives the
+// visible actions' indices; up to kFew of them are left to one warp, which reads
+// their scores and noise at once.  Rows with more than fit a list are taken by
+// the whole block afterwards.
+template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sample_masked_kernel(const __grid_constant__ SampleArgs a) {
+  constexpr int kRows = kMaskedThreads / 32, kIndices = 256;
+  __shared__ union {
+    Shared<kMaskedList> whole;
+    struct {
+      int index[kRows][kIndices], count[kRows];
+      union {
+        FewShared few[kRows];
+        uint64_t list[kRows][kIndices];
+      };
+    } part;
+  } sh;
+  const int teams = blockDim.x / (32 * a.row_warps), lanes = 32 * a.row_warps;
+  const int team_id = threadIdx.x / lanes, tid = threadIdx.x % lanes;
+  const int64_t row = a.first_row + (int64_t)blockIdx.x * teams + team_id;
+  const bool in = row < a.end_row;
+  const Row<T> r(a, in ? row : a.first_row);
+  if (tid == 0) sh.part.count[team_id] = 0;
+  if (lanes == 32) __syncwarp();
+  else __syncthreads();
+  if (in)
+    each_visible<10>(r, tid, lanes, [&](int first, uint32_t bits) {
+      int at = atomicAdd(&sh.part.count[team_id], __popc(bits));
+      for (; bits; bits &= bits - 1, ++at)
+        if (at < kIndices) sh.part.index[team_id][at] = first + __ffs(bits) - 1;
+    });
+  if (lanes == 32) __syncwarp();
+  else __syncthreads();
+  const int count = in ? sh.part.count[team_id] : 0;
+  if (in && tid < 32 && count <= kIndices) {
+    const Filters f(a.cfg, row);
+    const int* index = sh.part.index[team_id];
+    if (count <= kFew) {
+      int j[kMine];
+      float x[kMine];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        j[i] = tid + 32 * i < count ? index[tid + 32 * i] : -1;
+        x[i] = j[i] >= 0 ? to_f32(r.x[j[i]]) : -INFINITY;
+      }
+      draw_from_few(a, row, r, f, j, x, -1.0, sh.part.few[team_id]);
+    } else {
+      const Team<true> team{nullptr, tid, 32};
+      uint64_t* keys = sh.part.list[team_id];
+      uint64_t best = 0;
+      int seen = 0;
+      for (int i = tid; i < count; i += 32) {
+        const float x = to_f32(r.x[index[i]]);
+        const uint64_t key = x > -INFINITY ? rank_key(fminf(x, FLT_MAX), index[i]) : 0;
+        keys[i] = key;
+        seen += key != 0;
+        if (key > best) best = key;
+      }
+      best = team.max(best);
+      seen = team.sum(seen);
+      team.sync();
+      if (!best || f.greedy) {
+        if (tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
+      } else {
+        draw_from_list(a, row, team, r, f, keys, count, seen, key_score(best), -1.0);
+      }
+    }
+  }
+  const bool over = count > kIndices;
+  if (!__syncthreads_or(over)) return;
+  for (int t = 0; t < teams; ++t)
+    if (__syncthreads_or(over && team_id == t)) {
+      draw_masked_long<T>(a, a.first_row + (int64_t)blockIdx.x * teams + t, sh.whole);
+      __syncthreads();
+    }
+}
+
+// Rows of at most kList actions.
+template <typename T> __global__ void __launch_bounds__(kSampleThreads, 4) sample_list_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ Shared<kList> sh;
   const int64_t row = a.first_row + blockIdx.x;
   const int tid = threadIdx.x, n = blockDim.x;
   const Team<false> team{sh.slots, tid, n};
   const Row<T> r(a, row);
   uint64_t best = 0;
   int count = 0;
-  if (kMasked) {
-    if (tid == 0) sh.counter = 0;
-    __syncthreads();
-    each(r, tid, n, [&](int j, float x) {
-      const uint64_t key = rank_key(x, j);
-      if (key > best) best = key;
-      const int at = atomicAdd(&sh.counter, 1);
-      if (at < kList) sh.list[at] = key;
-    });
-  } else {
-    for (int j = tid; j < r.actions; j += n) {
-      const float v = to_f32(r.x[j]);
-      const uint64_t key = v > -INFINITY ? rank_key(fminf(v, FLT_MAX), j) : 0;
-      sh.list[j] = key;
-      count += key != 0;
-      if (key > best) best = key;
-    }
+  for (int j = tid; j < r.actions; j += n) {
+    const float v = to_f32(r.x[j]);
+    const uint64_t key = v > -INFINITY ? rank_key(fminf(v, FLT_MAX), j) : 0;
+    sh.list[j] = key;
+    count += key != 0;
+    if (key > best) best = key;
   }
   best = team.max(best);
   const Filters f(a.cfg, row);
@@ -552,21 +788,12 @@ __global__ void __launch_bounds__(kSampleThreads, 4) sample_list_kernel(const __
     if (tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
     return;
   }
-  count = kMasked ? sh.counter : team.sum(count);
-  const float top = key_score(best);
-  if (count > kList) {
-    __syncthreads();
-    draw_long_call<T, kMasked>(a, sh);
-  } else if (kMasked && count <= 64) {
-    if (tid < 32) draw_from_list(a, row, Team<true>{nullptr, tid, 32}, r, f, sh.list, count, count, top, -1.0);
-  } else {
-    draw_from_list(a, row, team, r, f, sh.list, kMasked ? count : r.actions, count, top, -1.0);
-  }
+  draw_from_list(a, row, team, r, f, sh.list, r.actions, team.sum(count), key_score(best), -1.0);
 }
 
 template <typename T> __global__ void __launch_bounds__(kSampleThreads, 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
-  __shared__ Shared sh;
-  draw_long<T, false>(a, sh);
+  __shared__ Shared<kList> sh;
+  draw_long<T, false>(a, a.first_row + blockIdx.x, sh);
 }
 
 template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cudaStream_t stream) {
@@ -579,12 +806,18 @@ template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cuda
     if (A <= kWarpRow) {
       sample_warp_kernel<T><<<(unsigned)((n + 3) / 4), 128, 0, stream>>>(a);
     } else {
-      // two mask groups of 16 a thread, or eight scores, or four vectors
-      const bool masked = a.rows.mask != nullptr, listed = A <= kList;
-      const int units = masked ? A / 32 : listed ? A / 8 : A / (4 * Row<T>::V);
-      const int threads = min(kSampleThreads, max(64, (units + 31) / 32 * 32));
-      auto kernel = masked ? sample_list_kernel<T, true> : listed ? sample_list_kernel<T, false> : sample_long_kernel<T>;
-      kernel<<<(unsigned)n, threads, 0, stream>>>(a);
+      // a warp for up to 5120 mask bytes (ten loads a lane), else the whole block;
+      // without a mask eight scores or four vectors a thread
+      if (a.rows.mask) {
+        a.row_warps = A <= 5120 ? 1 : kMaskedThreads / 32;
+        const int teams = kMaskedThreads / 32 / a.row_warps;
+        sample_masked_kernel<T><<<(unsigned)((n + teams - 1) / teams), kMaskedThreads, 0, stream>>>(a);
+      } else {
+        const int units = A <= kList ? A / 8 : A / (4 * Row<T>::V);
+        const int threads = min(kSampleThreads, max(64, (units + 31) / 32 * 32));
+        auto kernel = A <= kList ? sample_list_kernel<T> : sample_long_kernel<T>;
+        kernel<<<(unsigned)n, threads, 0, stream>>>(a);
+      }
     }
     e = cudaGetLastError();
   }
@@ -610,7 +843,7 @@ extern "C" gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sampl
   if (noise_stride < 0) return bad(who, "negative stride");
   if (rows->rows == 0) return GZ_OK;
   if (!d_action) return bad(who, "null actions");
-  const SampleArgs a{row_args(rows), *cfg, d_noise, noise_stride, d_action, d_logp, 0, 0};
+  const SampleArgs a{row_args(rows), *cfg, d_noise, noise_stride, d_action, d_logp, 0, 0, 1};
   const cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (rows->dtype == GZ_F32) e = launch_sample<float>(a, rows->rows, s);
