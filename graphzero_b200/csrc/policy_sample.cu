@@ -39,8 +39,6 @@ struct SampleArgs {
 };
 
 constexpr int kList = 2048;         // keys a block's list holds
-constexpr int kWarpRow = 256;       // actions of a row that a warp takes
-constexpr int kBins = 1024;         // of the histogram, which the list's memory holds
 constexpr int kMaskedList = 1024, kMaskedThreads = 128;  // the same for masked rows, and their blocks
 constexpr int kSampleThreads = 512;  // most threads of a block
 constexpr int64_t kRowsPerLaunch = 1 << 28;
@@ -326,7 +324,12 @@ __device__ __forceinline__ bool draw_from_few(const SampleArgs& a, int64_t row, 
     team.sync();
     int rank[kMine] = {};
     uint64_t before[kMine] = {}, sum = 0;
-    const int most = 32 - __clz(__ballot_sync(~0u, j[kMine - 1] >= 0)), full = most ? 32 * (kMine - 1) + most : 32;
+    int full = 0;  // keys lie below it
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const uint32_t some = __ballot_sync(~0u, key[i] != 0);
+      if (some) full = 32 * i + 32 - __clz(some);
+    }
     for (int q = 0; q < full; ++q) {
       const uint64_t k = sh.key[q], w = sh.weight[q];
 #pragma unroll
@@ -367,50 +370,23 @@ __device__ __forceinline__ bool draw_from_few(const SampleArgs& a, int64_t row, 
   return true;
 }
 
-// Rows of at most kWarpRow actions: a warp each, four a block.
+// Rows of at most kFew actions: a warp each, four a block.
 template <typename T> __global__ void __launch_bounds__(128) sample_warp_kernel(SampleArgs a) {
-  __shared__ uint64_t lists[4][kWarpRow];
   __shared__ FewShared few[4];
   const int64_t row = a.first_row + (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= a.end_row) return;
-  const Team<true> team{nullptr, (int)threadIdx.x % 32, 32};
+  const int lane = threadIdx.x % 32;
   const Row<T> r(a, row);
   const Filters f(a.cfg, row);
-  auto score = [&](int j) { return j < r.actions && !(r.mask && !r.mask[j]) ? to_f32(r.x[j]) : -INFINITY; };
-  if (r.actions <= kFew) {
-    int j[kMine];
-    float x[kMine];
+  int j[kMine];
+  float x[kMine];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      j[i] = team.tid + 32 * i < r.actions ? team.tid + 32 * i : -1;
-      x[i] = j[i] >= 0 ? score(j[i]) : -INFINITY;
-    }
-    draw_from_few(a, row, r, f, j, x, -1.0, few[threadIdx.x / 32]);
-    return;
+  for (int i = 0; i < kMine; ++i) {
+    const int k = lane + 32 * i;
+    j[i] = k < r.actions && !(r.mask && !r.mask[k]) ? k : -1;
+    x[i] = k < r.actions ? to_f32(r.x[k]) : -INFINITY;
   }
-  uint64_t* keys = lists[threadIdx.x / 32];
-  uint64_t best = 0;
-  int count = 0;
-#pragma unroll 2
-  for (int j0 = 0; j0 < r.actions; j0 += 32) {
-    const int j = j0 + team.tid;
-    const float v = score(j);
-    const bool in = v > -INFINITY;
-    const uint32_t all = __ballot_sync(~0u, in);
-    if (in) {
-      const uint64_t key = rank_key(fminf(v, FLT_MAX), j);
-      keys[count + __popc(all & ((1u << team.tid) - 1))] = key;
-      if (key > best) best = key;
-    }
-    count += __popc(all);
-  }
-  best = team.max(best);
-  team.sync();
-  if (!best || f.greedy) {
-    if (team.tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
-    return;
-  }
-  draw_from_list(a, row, team, r, f, keys, count, count, key_score(best), -1.0);
+  draw_from_few(a, row, r, f, j, x, -1.0, few[threadIdx.x / 32]);
 }
 
 // The rank key of the last kept action: the largest with at least `goal` (a
@@ -429,36 +405,42 @@ __device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, cons
   return last;
 }
 
-// The same through a histogram of kBins bins over the 31 temperatures below the
-// best score (what lies deeper, by bisection if need be).
+// The same through a histogram, in the list's memory, over the 31 temperatures
+// below the best score (what lies deeper is found by bisection if need be).
 template <bool kWeights, int kSize, typename T>
 __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal,
                                               uint64_t* memory, int* counter) {
   __shared__ uint64_t above;
   __shared__ int found;
-  unsigned long long* bins = (unsigned long long*)memory;
+  constexpr int kBins = kSize;
+  uint32_t *low = (uint32_t*)memory, *high = low + kBins;
   const float scale = kBins / (31.f * f.temperature);
   auto bin = [&](float x) { return min(kBins - 1, (int)((top - x) * scale)); };  // falls as x rises, weakly
   team.sync();
-  for (int i = team.tid; i < kBins; i += team.n) bins[i] = 0;
+  for (int i = team.tid; i < kBins; i += team.n) low[i] = high[i] = 0;
   if (team.tid == 0) *counter = 0, found = kBins;
   team.sync();
   each(r, team.tid, team.n, [&](int, float x) {
-    const unsigned long long w = kWeights ? fixed_weight(expf(f.depth(x, top))) : 1ull;
-    if (w) atomicAdd(&bins[bin(x)], w);
+    const uint64_t w = kWeights ? fixed_weight(expf(f.depth(x, top))) : 1;
+    if (!w) return;
+    // in two halves, for only 32-bit adds are done in shared memory at once
+    const int b = bin(x);
+    const uint32_t old = atomicAdd(&low[b], (uint32_t)w), up = (uint32_t)(w >> 32) + (old + (uint32_t)w < old);
+    if (up) atomicAdd(&high[b], up);
   });
   team.sync();
   const int per = kBins / team.n, lo = team.tid * per;  // n divides kBins or the rest is the last thread's
   const int hi = team.tid == team.n - 1 ? kBins : lo + per;
   uint64_t mine = 0;
-  for (int i = lo; i < hi; ++i) mine += bins[i];
+  auto weight = [&](int i) { return (uint64_t)high[i] << 32 | low[i]; };
+  for (int i = lo; i < hi; ++i) mine += weight(i);
   uint64_t sum = team.before(mine);
   for (int i = lo; i < hi; ++i) {
-    if ((double)sum < goal && (double)(sum + bins[i]) >= goal) {
+    if ((double)sum < goal && (double)(sum + weight(i)) >= goal) {
       found = i;
       above = sum;
     }
-    sum += bins[i];
+    sum += weight(i);
   }
   team.sync();
   const int b = found;
@@ -485,6 +467,82 @@ template <int kSize> struct Shared {
   uint64_t slots[kSampleThreads / 32], list[kSize];
   int counter;
 };
+
+// Draws from all of an unmasked row: the scores from the caches once more, and
+// the noise.  The row's weight is taken in 32 bits.
+template <typename T>
+__device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T>& r, const Filters& f, float top) {
+  constexpr int V = Row<T>::V;
+  const int tid = team.tid, n = team.n;
+  const float* noise = r.noise ? r.noise + r.head : nullptr;
+  const bool aligned = ((uintptr_t)noise & 15) == 0;
+  float most = -INFINITY, z = 0.f;
+  int where = -1;  // vector of the best noisy score, or actions + the index of a score beside the vectors
+  auto scores = [&](int v, float* s, float* d) {
+    unpack<T>(r.vector(v), d);
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (noise) {
+        const float* p = noise + v * V + k;
+        g = aligned ? __ldg((const float4*)p) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float x = d[k + q];
+        d[k + q] = x > -INFINITY ? f.depth(fminf(x, FLT_MAX), top) : -INFINITY;
+        s[k + q] = d[k + q] + (&g.x)[q];
+      }
+    }
+  };
+#pragma unroll 2
+  for (int v = tid; v < r.vecs; v += n) {
+    float s[V], d[V];
+    scores(v, s, d);
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      z += sm100::ex2_approx(d[k] * 1.44269504f);
+      m = fmaxf(m, s[k]);
+    }
+    if (m > most) {
+      most = m;
+      where = v;
+    }
+  }
+  uint64_t best = 0;
+  if (where >= 0) {
+    float s[V], d[V];
+    scores(where, s, d);
+#pragma unroll
+    for (int k = V - 1; k >= 0; --k)
+      if (s[k] == most) best = rank_key(most, r.head + where * V + k);
+  }
+  if (tid < r.ends) {
+    const int j = r.end_index(tid);
+    const float x = to_f32(r.x[j]);
+    if (x > -INFINITY) {
+      const float d = f.depth(fminf(x, FLT_MAX), top), s = d + (r.noise ? r.noise[j] : 0.f);
+      z += sm100::ex2_approx(d * 1.44269504f);
+      const uint64_t key = rank_key(s >= -INFINITY ? s : -INFINITY, j);
+      if (key > best) best = key;
+    }
+  }
+  z = team.sum(z);
+  best = team.max(best);
+  if (key_score(best) == -INFINITY || !best) {  // no score above -inf: the first visible action
+    best = 0;
+    each(r, tid, n, [&](int j, float) {
+      const uint64_t key = rank_key(-INFINITY, j);
+      if (key > best) best = key;
+    });
+    best = team.max(best);
+  }
+  if (tid == 0) {
+    const int j = key_index(best);
+    answer(a, row, j, f.depth(fminf(to_f32(r.x[j]), FLT_MAX), top) - logf(z));
+  }
+}
 
 // A row whose visible actions do not all fit the list.
 template <typename T, bool kMasked, int kSize>
@@ -678,11 +736,17 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       if (cut > last) last = cut;
     }
   }
-  Draw d;
-  each(r, tid, n, [&](int j, float x) {
-    if (rank_key(x, j) >= last) d.add(f, top, x, j, r.noise);
-  });
-  d.finish(a, row, team, r, f, top);
+  if (kMasked || last || f.min_p > 0.f) {
+    const float score = last ? key_score(last) : -INFINITY, floor = f.min_p > 0.f ? logf(f.min_p) - 0.01f : -INFINITY;
+    Draw d;
+    each(r, tid, n, [&](int j, float x) {
+      if (x < score || (x == score && j > key_index(last)) || (x - top) < floor * f.temperature * 1.01f) return;
+      d.add(f, top, x, j, r.noise);
+    });
+    d.finish(a, row, team, r, f, top);
+    return;
+  }
+  draw_from_all(a, row, team, r, f, top);
 }
 
 // A call of its own, so that rows that fit the list do not pay for its registers.
@@ -699,33 +763,33 @@ template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sampl
   __shared__ union {
     Shared<kMaskedList> whole;
     struct {
-      int index[kRows][kIndices], count[kRows];
+      int index[kIndices], count;
       union {
-        FewShared few[kRows];
-        uint64_t list[kRows][kIndices];
+        FewShared few;
+        uint64_t list[kIndices];
       };
-    } part;
+    } part[kRows];
   } sh;
   const int teams = blockDim.x / (32 * a.row_warps), lanes = 32 * a.row_warps;
   const int team_id = threadIdx.x / lanes, tid = threadIdx.x % lanes;
   const int64_t row = a.first_row + (int64_t)blockIdx.x * teams + team_id;
   const bool in = row < a.end_row;
   const Row<T> r(a, in ? row : a.first_row);
-  if (tid == 0) sh.part.count[team_id] = 0;
+  if (tid == 0) sh.part[team_id].count = 0;
   if (lanes == 32) __syncwarp();
   else __syncthreads();
   if (in)
     each_visible<10>(r, tid, lanes, [&](int first, uint32_t bits) {
-      int at = atomicAdd(&sh.part.count[team_id], __popc(bits));
+      int at = atomicAdd(&sh.part[team_id].count, __popc(bits));
       for (; bits; bits &= bits - 1, ++at)
-        if (at < kIndices) sh.part.index[team_id][at] = first + __ffs(bits) - 1;
+        if (at < kIndices) sh.part[team_id].index[at] = first + __ffs(bits) - 1;
     });
   if (lanes == 32) __syncwarp();
   else __syncthreads();
-  const int count = in ? sh.part.count[team_id] : 0;
+  const int count = in ? sh.part[team_id].count : 0;
   if (in && tid < 32 && count <= kIndices) {
     const Filters f(a.cfg, row);
-    const int* index = sh.part.index[team_id];
+    const int* index = sh.part[team_id].index;
     if (count <= kFew) {
       int j[kMine];
       float x[kMine];
@@ -734,10 +798,10 @@ template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sampl
         j[i] = tid + 32 * i < count ? index[tid + 32 * i] : -1;
         x[i] = j[i] >= 0 ? to_f32(r.x[j[i]]) : -INFINITY;
       }
-      draw_from_few(a, row, r, f, j, x, -1.0, sh.part.few[team_id]);
+      draw_from_few(a, row, r, f, j, x, -1.0, sh.part[team_id].few);
     } else {
       const Team<true> team{nullptr, tid, 32};
-      uint64_t* keys = sh.part.list[team_id];
+      uint64_t* keys = sh.part[team_id].list;
       uint64_t best = 0;
       int seen = 0;
       for (int i = tid; i < count; i += 32) {
@@ -766,33 +830,9 @@ template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sampl
     }
 }
 
-// Rows of at most kList actions.
-template <typename T> __global__ void __launch_bounds__(kSampleThreads, 4) sample_list_kernel(const __grid_constant__ SampleArgs a) {
-  __shared__ Shared<kList> sh;
-  const int64_t row = a.first_row + blockIdx.x;
-  const int tid = threadIdx.x, n = blockDim.x;
-  const Team<false> team{sh.slots, tid, n};
-  const Row<T> r(a, row);
-  uint64_t best = 0;
-  int count = 0;
-  for (int j = tid; j < r.actions; j += n) {
-    const float v = to_f32(r.x[j]);
-    const uint64_t key = v > -INFINITY ? rank_key(fminf(v, FLT_MAX), j) : 0;
-    sh.list[j] = key;
-    count += key != 0;
-    if (key > best) best = key;
-  }
-  best = team.max(best);
-  const Filters f(a.cfg, row);
-  if (!best || f.greedy) {
-    if (tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
-    return;
-  }
-  draw_from_list(a, row, team, r, f, sh.list, r.actions, team.sum(count), key_score(best), -1.0);
-}
-
-template <typename T> __global__ void __launch_bounds__(kSampleThreads, 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
-  __shared__ Shared<kList> sh;
+template <typename T, int kSize, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_long_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ Shared<kSize> sh;
   draw_long<T, false>(a, a.first_row + blockIdx.x, sh);
 }
 
@@ -803,7 +843,7 @@ template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cuda
     a.first_row = first;
     a.end_row = first + n;
     const int A = a.rows.actions;
-    if (A <= kWarpRow) {
+    if (A <= kFew) {
       sample_warp_kernel<T><<<(unsigned)((n + 3) / 4), 128, 0, stream>>>(a);
     } else {
       // a warp for up to 5120 mask bytes (ten loads a lane), else the whole block;
@@ -813,10 +853,10 @@ template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cuda
         const int teams = kMaskedThreads / 32 / a.row_warps;
         sample_masked_kernel<T><<<(unsigned)((n + teams - 1) / teams), kMaskedThreads, 0, stream>>>(a);
       } else {
-        const int units = A <= kList ? A / 8 : A / (4 * Row<T>::V);
-        const int threads = min(kSampleThreads, max(64, (units + 31) / 32 * 32));
-        auto kernel = A <= kList ? sample_list_kernel<T> : sample_long_kernel<T>;
-        kernel<<<(unsigned)n, threads, 0, stream>>>(a);
+        // 32 scores a thread, so that there are many best scores to choose from
+        const int threads = min(kSampleThreads, max(32, (A / 32 + 31) / 32 * 32));
+        if (threads <= 64) sample_long_kernel<T, 512, 64><<<(unsigned)n, threads, 0, stream>>>(a);
+        else sample_long_kernel<T, kList, kSampleThreads><<<(unsigned)n, threads, 0, stream>>>(a);
       }
     }
     e = cudaGetLastError();
