@@ -13,7 +13,9 @@ broadcast_weights) and its factory create_neural_net(type, game)
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -162,9 +164,8 @@ _SIGS = {
     "gz_train_batch_indices": (C.c_int, [C.c_int64, C.POINTER(TrainConfig), C.c_int, C.c_int64, C.c_int, C.c_int,
                                          C.POINTER(C.c_int64)]),
     "gz_train_bucket_range": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
-    "gz_policy_sample": (C.c_int, [C.POINTER(PolicyRows), C.POINTER(SampleConfig), _vp, C.c_int64, _vp, _vp, _vp]),
-    "gz_policy_loss": (C.c_int, [C.POINTER(PolicyRows), _vp, C.c_int64, _vp, _vp, C.c_float, _vp, _vp, C.c_int64,
-                                 _vp]),
+    "gz_policy_sample": (C.c_int, [_vp, _vp, _vp, C.c_int64, _vp, _vp, _vp]),
+    "gz_policy_loss": (C.c_int, [_vp, _vp, C.c_int64, _vp, _vp, C.c_float, _vp, _vp, C.c_int64, _vp]),
     "gz_adamw_create": (C.c_int, [C.POINTER(AdamWTensor), C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
     "gz_adamw_destroy": (C.c_int, [_vp]),
     "gz_adamw_step": (C.c_int, [_vp, C.POINTER(_vp), _i32p, C.POINTER(AdamWConfig), _vp, _vp]),
@@ -695,22 +696,79 @@ def load_train_examples(path) -> list:
 # ---- policies of the caller's own: drawing actions, loss, optimiser (gz_policy_*, gz_adamw_*) ----
 
 
+# gz_policy_rows and gz_sample_config are packed here rather than built as
+# ctypes structures: the small calls' time is the host's.
+_PACK_ROWS, _PACK_SAMPLE = struct.Struct("PPqqqii"), struct.Struct("fffiPPPP")
+assert _PACK_ROWS.size == C.sizeof(PolicyRows) and _PACK_SAMPLE.size == C.sizeof(SampleConfig)
+_torch = None  # imported by the first call that needs it
+_float_dtypes = {}  # torch type -> gz_dtype
+
+
+def _need_torch():
+    global _torch
+    if _torch is None:
+        import torch
+        _float_dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _torch = torch
+    return _torch
+
+
+def _current_stream(device) -> int:
+    """Raw handle of the device's current stream."""
+    return _torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _On:
+    """A device as the current one, and a stream of it as its current stream, for
+    the scope (so that what is allocated and copied there is ordered with it)."""
+
+    def __init__(self, device, stream):
+        if isinstance(stream, int):
+            stream = _torch.cuda.ExternalStream(stream, device=device)
+        self._device, self._stream = _torch.cuda.device(device), stream and _torch.cuda.stream(stream)
+
+    def __enter__(self):
+        self._device.__enter__()
+        if self._stream:
+            self._stream.__enter__()
+
+    def __exit__(self, *exc):
+        if self._stream:
+            self._stream.__exit__(*exc)
+        self._device.__exit__(*exc)
+
+
+def _on(f):
+    """Runs f(tensor, ..., stream=...) with the tensor's device and the stream current."""
+
+    @functools.wraps(f)
+    def run(x, *args, stream=None, **kw):
+        torch = _torch or _need_torch()
+        if stream is None and (not x.is_cuda or x.device.index == torch._C._cuda_getDevice()):
+            return f(x, *args, **kw)
+        if not x.is_cuda:
+            raise ValueError("CUDA tensors are needed")
+        with _On(x.device, stream):
+            return f(x, *args, **kw)
+
+    return run
+
+
 def _policy_rows(logits, mask):
-    """gz_policy_rows of torch tensors [rows][actions] (and what it points to)."""
-    import torch
-    dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if logits.dim() != 2 or logits.dtype not in dtypes or not logits.is_cuda:
+    """What gz_policy_rows points to, and its packed form."""
+    dtype = _float_dtypes.get(logits.dtype)
+    if dtype is None or logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("logits must be a [rows][actions] CUDA tensor of float32, float16 or bfloat16")
     n, a = logits.shape
     if a > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
-    if mask is not None:
-        if mask.shape != logits.shape or mask.dtype not in (torch.uint8, torch.bool) or mask.device != logits.device:
-            raise ValueError("mask must be a uint8 or bool tensor of the logits' shape and device")
-        if a > 1 and mask.stride(1) != 1:
-            mask = mask.contiguous()
-    return logits, mask, PolicyRows(logits.data_ptr(), None if mask is None else mask.data_ptr(), logits.stride(0),
-                                    0 if mask is None else mask.stride(0), n, a, dtypes[logits.dtype])
+    if mask is None:
+        return logits, None, _PACK_ROWS.pack(logits.data_ptr(), 0, logits.stride(0), 0, n, a, dtype)
+    if mask.shape != logits.shape or mask.dtype not in (_torch.uint8, _torch.bool) or mask.device != logits.device:
+        raise ValueError("mask must be a uint8 or bool tensor of the logits' shape and device")
+    if a > 1 and mask.stride(1) != 1:
+        mask = mask.contiguous()
+    return logits, mask, _PACK_ROWS.pack(logits.data_ptr(), mask.data_ptr(), logits.stride(0), mask.stride(0), n, a, dtype)
 
 
 def _row_values(x, name, dtype, n, device):
@@ -720,31 +778,15 @@ def _row_values(x, name, dtype, n, device):
     return x.contiguous()
 
 
-def _action_values(x, name, shape, device):
+def _action_values(x, name, logits):
     """A float32 [rows][actions] tensor whose rows are contiguous."""
-    import torch
-    if x.shape != shape or x.dtype != torch.float32 or x.device != device:
+    if x.shape != logits.shape or x.dtype != _torch.float32 or x.device != logits.device:
         raise ValueError(f"{name} must be a float32 tensor of the logits' shape and device")
-    return x if shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-class _On:
-    """The tensor's device for the scope, entered only where it is not the current one."""
-
-    def __init__(self, device):
-        import torch
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-
-
-def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=None):
+@_on
+def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One action per row of `logits` (torch, [rows][actions], float32, float16
     or bfloat16), drawn with `noise` (float32 standard Gumbel numbers of the
     same shape, e.g. -torch.empty(...).exponential_().log(); None picks the
@@ -752,52 +794,63 @@ def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p
     temperature, top_k, top_p and min_p keep.  Each setting is a number or a
     [rows] tensor (float32; top_k int32).  Returns (action int32 [rows], -1
     where nothing is visible; logp float32 [rows], the action's
-    log-probability among the kept ones).  See gz_policy_sample."""
-    import torch
+    log-probability among the kept ones).  `stream` (keyword): a stream to run
+    on instead of the current one.  See gz_policy_sample."""
     logits, mask, rows = _policy_rows(logits, mask)
-    n, dev, cfg = logits.shape[0], logits.device, SampleConfig(1.0, 1.0, 0.0, 0)
-    kept = []  # what the settings point to
-    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(x, torch.Tensor):
-            kept.append(_row_values(x, name, dtype, n, dev))
-            setattr(cfg, "d_" + name, kept[-1].data_ptr())
-        else:
-            setattr(cfg, name, x)
+    n, dev, tensor = logits.shape[0], logits.device, _torch.Tensor
+    d_temperature = d_top_k = d_top_p = d_min_p = 0
+    if isinstance(temperature, tensor):
+        temperature_rows = _row_values(temperature, "temperature", _torch.float32, n, dev)
+        temperature, d_temperature = 1.0, temperature_rows.data_ptr()
+    if isinstance(top_k, tensor):
+        top_k_rows = _row_values(top_k, "top_k", _torch.int32, n, dev)
+        top_k, d_top_k = 0, top_k_rows.data_ptr()
+    if isinstance(top_p, tensor):
+        top_p_rows = _row_values(top_p, "top_p", _torch.float32, n, dev)
+        top_p, d_top_p = 1.0, top_p_rows.data_ptr()
+    if isinstance(min_p, tensor):
+        min_p_rows = _row_values(min_p, "min_p", _torch.float32, n, dev)
+        min_p, d_min_p = 0.0, min_p_rows.data_ptr()
+    cfg = _PACK_SAMPLE.pack(temperature, top_p, min_p, min(top_k, 0x7fffffff), d_temperature, d_top_p, d_min_p, d_top_k)
     if noise is not None:
-        noise = _action_values(noise, "noise", logits.shape, dev)
-    action = torch.empty(n, dtype=torch.int32, device=dev)
-    logp = torch.empty(n, dtype=torch.float32, device=dev)
-    with _On(dev):
-        _check(_lib.gz_policy_sample(C.byref(rows), C.byref(cfg), _dev(noise), 0 if noise is None else noise.stride(0),
-                                     action.data_ptr(), logp.data_ptr(), _stream(stream)))
+        noise = _action_values(noise, "noise", logits)
+    action, logp = logits.new_empty(n, dtype=_torch.int32), logits.new_empty(n, dtype=_torch.float32)
+    status = _lib.gz_policy_sample(rows, cfg, noise if noise is None else noise.data_ptr(),
+                                   0 if noise is None else noise.stride(0), action.data_ptr(), logp.data_ptr(),
+                                   _current_stream(dev))
+    if status:
+        _check(status)
     return action, logp
 
 
-def policy_loss(logits, target=None, label=None, mask=None, weight=None, grad_scale=1.0, need_grad=True, stream=None):
+@_on
+def policy_loss(logits, target=None, label=None, mask=None, weight=None, grad_scale=1.0, need_grad=True):
     """Cross-entropy of softmax(logits) over the actions that `mask` leaves
     visible, and its gradient, in one pass: (loss float32 [rows], grad of the
     logits' shape and type, or None without need_grad).  The targets are
     `target` (float32 [rows][actions] amounts) or `label` (int32 [rows]);
     `weight` (float32 [rows]) multiplies a row, `grad_scale` the gradient
     alone (1 / rows for the mean loss).  Continue a torch backward pass with
-    logits.backward(grad).  See gz_policy_loss."""
-    import torch
+    logits.backward(grad).  `stream` (keyword): a stream to run on instead of
+    the current one.  See gz_policy_loss."""
     logits, mask, rows = _policy_rows(logits, mask)
     (n, a), dev = logits.shape, logits.device
     if (target is None) == (label is None):
         raise ValueError("give either target or label")
     if target is not None:
-        target = _action_values(target, "target", logits.shape, dev)
+        target = _action_values(target, "target", logits)
     else:
-        label = _row_values(label, "label", torch.int32, n, dev)
+        label = _row_values(label, "label", _torch.int32, n, dev)
     if weight is not None:
-        weight = _row_values(weight, "weight", torch.float32, n, dev)
-    loss = torch.empty(n, dtype=torch.float32, device=dev)
-    grad = torch.empty((n, a), dtype=logits.dtype, device=dev) if need_grad else None
-    with _On(dev):
-        _check(_lib.gz_policy_loss(C.byref(rows), _dev(target), 0 if target is None else target.stride(0), _dev(label),
-                                   _dev(weight), grad_scale, loss.data_ptr(), _dev(grad), a, _stream(stream)))
+        weight = _row_values(weight, "weight", _torch.float32, n, dev)
+    loss = logits.new_empty(n, dtype=_torch.float32)
+    grad = logits.new_empty((n, a)) if need_grad else None
+    status = _lib.gz_policy_loss(rows, target if target is None else target.data_ptr(),
+                                 0 if target is None else target.stride(0), label if label is None else label.data_ptr(),
+                                 weight if weight is None else weight.data_ptr(), grad_scale, loss.data_ptr(),
+                                 grad if grad is None else grad.data_ptr(), a, _current_stream(dev))
+    if status:
+        _check(status)
     return loss, grad
 
 
@@ -816,7 +869,7 @@ class AdamW:
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, copies=None,
                  lr_scale=1.0, max_norm=0.0, seed=0):
-        import torch
+        torch = _need_torch()
         self._plan = _vp()
         self.params = list(params)
         count = len(self.params)
@@ -846,7 +899,6 @@ class AdamW:
             self.m, self.v = self.m.to(torch.float8_e4m3fn), self.v.to(torch.float8_e4m3fn)
             self.m_scale = torch.ones(total // ADAMW_BLOCK, device=self.device)
             self.v_scale = torch.ones(total // ADAMW_BLOCK, device=self.device)
-        self._dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
         table = (AdamWTensor * count)()
         size = self.m.element_size()
         for t, p, c, at, decay, scale in zip(table, self.params, self.copies, self.offsets, decays, scales):
@@ -856,8 +908,9 @@ class AdamW:
                 t.m_scale = self.m_scale.data_ptr() + at // ADAMW_BLOCK * 4
                 t.v_scale = self.v_scale.data_ptr() + at // ADAMW_BLOCK * 4
             if c is not None:
-                t.copy, t.copy_dtype = c.data_ptr(), self._dtypes[c.dtype]
+                t.copy, t.copy_dtype = c.data_ptr(), _float_dtypes[c.dtype]
         _check(_lib.gz_adamw_create(table, count, state_bits, self.device.index, C.byref(self._plan)))
+        self._shapes = [p.shape for p in self.params]
         self._grads, self._kinds, self._cfg = (_vp * count)(), (C.c_int32 * count)(), AdamWConfig()
 
     def close(self) -> None:
@@ -877,26 +930,32 @@ class AdamW:
         weights' .grad by default), each multiplied by grad_scale.  Returns
         their global norm (a float32 device tensor) with max_norm > 0, else
         None."""
-        import torch
         if grads is None:
             grads = [p.grad for p in self.params]
         if len(grads) != len(self.params):
             raise ValueError("grads needs one entry per tensor")
-        for k, (g, p) in enumerate(zip(grads, self.params)):
+        pointers, kinds, device, dtypes = self._grads, self._kinds, self.device, _float_dtypes
+        for k, g in enumerate(grads):
             if g is None:
-                self._grads[k] = None
+                pointers[k] = None
                 continue
-            kind = self._dtypes.get(g.dtype)
-            if kind is None or g.shape != p.shape or g.device != self.device or not g.is_contiguous():
+            kind = dtypes.get(g.dtype)
+            if kind is None or g.shape != self._shapes[k] or g.device != device or not g.is_contiguous():
                 raise ValueError("gradients must be contiguous tensors of their weights' shapes in float32, float16 "
                                  "or bfloat16")
-            self._grads[k], self._kinds[k] = g.data_ptr(), kind
-        norm = torch.empty((), device=self.device) if self.max_norm > 0 else None
+            pointers[k], kinds[k] = g.data_ptr(), kind
+        if stream is None and device.index == _torch._C._cuda_getDevice():
+            return self._step(grad_scale)
+        with _On(device, stream):
+            return self._step(grad_scale)
+
+    def _step(self, grad_scale):
+        norm = _torch.empty((), device=self.device) if self.max_norm > 0 else None
         c = self._cfg
         c.lr, (c.beta1, c.beta2), c.eps = self.lr, self.betas, self.eps
         c.max_norm, c.grad_scale, c.step, c.seed = self.max_norm, grad_scale, self.steps + 1, self.seed
-        with _On(self.device):
-            _check(_lib.gz_adamw_step(self._plan, self._grads, self._kinds, C.byref(c), _dev(norm), _stream(stream)))
+        _check(_lib.gz_adamw_step(self._plan, self._grads, self._kinds, C.byref(c), norm if norm is None else norm.data_ptr(),
+                                  _current_stream(self.device)))
         self.steps += 1
         return norm
 
