@@ -41,6 +41,8 @@ struct SampleArgs {
 constexpr int kList = 2048;         // keys a block's list holds
 constexpr int kMaskedList = 1024, kMaskedThreads = 128;  // the same for masked rows, and their blocks
 constexpr int kSampleThreads = 512;  // most threads of a block
+constexpr int kReachBit = 16;       // lowest bit of a score that the search for a list's bound looks at
+constexpr int kMaximaVecs = 24576;  // vectors of a row whose maxima are kept (96 KB: two blocks fit an SM)
 constexpr int64_t kRowsPerLaunch = 1 << 28;
 
 // exp(d) in units of 2^-44 (d <= 0): 2^18 actions sum below 2^63.
@@ -407,9 +409,10 @@ __device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, cons
 
 // The same through a histogram, in the list's memory, over the 31 temperatures
 // below the best score (what lies deeper is found by bisection if need be).
+// Scores below `from` are known not to be kept.
 template <bool kWeights, int kSize, typename T>
 __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal,
-                                              uint64_t* memory, int* counter) {
+                                              float from, uint64_t* memory, int* counter) {
   __shared__ uint64_t above;
   __shared__ int found;
   constexpr int kBins = kSize;
@@ -421,6 +424,7 @@ __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row
   if (team.tid == 0) *counter = 0, found = kBins;
   team.sync();
   each(r, team.tid, team.n, [&](int, float x) {
+    if (x < from) return;
     const uint64_t w = kWeights ? fixed_weight(expf(f.depth(x, top))) : 1;
     if (!w) return;
     // in two halves, for only 32-bit adds are done in shared memory at once
@@ -545,8 +549,9 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
 }
 
 // A row whose visible actions do not all fit the list.
+// maxima: a float for every vector of the row, or null.
 template <typename T, bool kMasked, int kSize>
-__device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh) {
+__device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh, float* maxima) {
   constexpr int V = Row<T>::V;
   const int tid = threadIdx.x, n = blockDim.x;
   const Team<false> team{sh.slots, tid, n};
@@ -580,6 +585,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       for (int i = 0; i < kAhead; ++i) {
         if (v0 + i * n >= r.vecs) continue;
         const float m = fminf(max_vector<false, T>(-INFINITY, raw[i], 0), FLT_MAX);
+        if (maxima) maxima[v0 + i * n] = m;
         if (m > most) {
           most = m;
           where = v0 + i * n;
@@ -642,7 +648,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
     // The largest number that enough threads' best scores reach: top_k of them;
     // or so many that they weigh top_p of the row, or else half of them, which
     // with what lies between them may still be enough.  One warp searches for
-    // it, over the scores' upper 20 bits, with weights in units of 2^-22.
+    // it, over the scores' upper 16 bits, with weights in units of 2^-22.
     if (!by_count || f.top_k <= n) {
       uint32_t* scores = (uint32_t*)sh.list;
       scores[tid] = (uint32_t)(mine >> 18);
@@ -660,21 +666,36 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
           for (int i = 0; i < kSampleThreads / 32; ++i) c += score[i] >= mid ? weight[i] : 0;
           return __reduce_add_sync(~0u, c);
         };
+        uint32_t least = ~0u, most = 0;
+#pragma unroll
+        for (int i = 0; i < kSampleThreads / 32; ++i)
+          if (score[i]) {
+            least = min(least, score[i]);
+            most = max(most, score[i]);
+          }
+        least = __reduce_min_sync(~0u, least);
+        most = __reduce_max_sync(~0u, most);
         uint32_t goal = f.top_k;
         if (!by_count) {
           const double g = f.top_p * row_weight * 0x1p-22 * 1.00001 + 1;
           goal = g < 0x1p31 ? (uint32_t)g : ~0u;
-          if (above(1) < goal) {
+          const uint32_t all = above(1);
+          if (all < goal / 2) {
+            goal = ~0u;  // hopeless
+          } else if (all < goal) {
             goal = n / 2;
 #pragma unroll
             for (int i = 0; i < kSampleThreads / 32; ++i) weight[i] = 1;
           }
         }
-        uint32_t most = 0;
+        // the bits that all scores share need no search
+        const int first = 31 - __clz(least ^ most | 1);
+        uint32_t reach = above(1) >= goal ? most & ~((2u << first) - 1) : 0;
+        if (reach)
 #pragma unroll 1
-        for (int bit = 31; bit >= 12; --bit)
-          if (above(most | 1u << bit) >= goal) most |= 1u << bit;
-        if (tid == 0) *(uint32_t*)sh.slots = most;
+          for (int bit = first; bit >= kReachBit; --bit)
+            if (above(reach | 1u << bit) >= goal) reach |= 1u << bit;
+        if (tid == 0) *(uint32_t*)sh.slots = reach;
       }
       __syncthreads();
       const uint32_t reach = *(uint32_t*)sh.slots;
@@ -692,15 +713,28 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
           each(r, tid, n, take);
         } else {
           if (tid < r.ends) take(r.end_index(tid), fminf(to_f32(r.x[r.end_index(tid)]), FLT_MAX));
-#pragma unroll 4
-          for (int v = tid; v < r.vecs; v += n) {
-            const uint4 raw = r.vector(v);
-            if (max_vector<false, T>(-INFINITY, raw, 0) < from) continue;
+          auto take_vector = [&](int v, uint4 raw) {
             float x[V];
             unpack<T>(raw, x);
 #pragma unroll
             for (int k = 0; k < V; ++k)
               if (x[k] == x[k]) take(r.head + v * V + k, fminf(x[k], FLT_MAX));
+          };
+          if (maxima) {  // each thread the vectors that it has read
+#pragma unroll 4
+            for (int v = tid; v < r.vecs; v += n)
+              if (maxima[v] >= from) take_vector(v, r.vector(v));
+          } else {
+            constexpr int kAhead = 4;
+            for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
+              uint4 raw[kAhead];
+#pragma unroll
+              for (int i = 0; i < kAhead; ++i)
+                if (v0 + i * n < r.vecs) raw[i] = r.vector(v0 + i * n);
+#pragma unroll
+              for (int i = 0; i < kAhead; ++i)
+                if (v0 + i * n < r.vecs && max_vector<false, T>(-INFINITY, raw[i], 0) >= from) take_vector(v0 + i * n, raw[i]);
+            }
           }
         }
         __syncthreads();
@@ -723,7 +757,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
         } else if (m <= kSize && draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
       }
     }
-    if (by_count) last = last_by_bins<false, kSize>(team, r, f, top, (double)f.top_k, sh.list, &sh.counter);
+    if (by_count) last = last_by_bins<false, kSize>(team, r, f, top, (double)f.top_k, -INFINITY, sh.list, &sh.counter);
     if (by_weight) {
       if (by_count) {
         uint64_t w = 0;
@@ -732,7 +766,11 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
         });
         row_weight = (double)team.sum(w);
       }
-      const uint64_t cut = last_by_bins<true, kSize>(team, r, f, top, f.top_p * row_weight, sh.list, &sh.counter);
+      // all actions of less than (1 - top_p) / actions of the weight have less
+      // than 1 - top_p of it together: the share is reached before them
+      const float least = (float)((1.0 - f.top_p) * row_weight * 0x1p-44) / r.actions * 0.999f;
+      const float from = least > 1e-30f ? top + (logf(fminf(least, 1.f)) - 0.001f) * f.temperature : -INFINITY;
+      const uint64_t cut = last_by_bins<true, kSize>(team, r, f, top, f.top_p * row_weight, from, sh.list, &sh.counter);
       if (cut > last) last = cut;
     }
   }
@@ -751,7 +789,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
 
 // A call of its own, so that rows that fit the list do not pay for its registers.
 template <typename T, int kSize> __device__ __noinline__ void draw_masked_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh) {
-  draw_long<T, true>(a, row, sh);
+  draw_long<T, true>(a, row, sh, nullptr);
 }
 
 // Masked rows, in blocks of `row_warps` warps for every row: the mask gives the
@@ -833,7 +871,8 @@ template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sampl
 template <typename T, int kSize, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_long_kernel(const __grid_constant__ SampleArgs a) {
   __shared__ Shared<kSize> sh;
-  draw_long<T, false>(a, a.first_row + blockIdx.x, sh);
+  extern __shared__ float maxima[];
+  draw_long<T, false>(a, a.first_row + blockIdx.x, sh, a.rows.actions / Row<T>::V <= kMaximaVecs ? maxima : nullptr);
 }
 
 template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cudaStream_t stream) {
@@ -855,8 +894,17 @@ template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cuda
       } else {
         // 32 scores a thread, so that there are many best scores to choose from
         const int threads = min(kSampleThreads, max(32, (A / 32 + 31) / 32 * 32));
-        if (threads <= 64) sample_long_kernel<T, 512, 64><<<(unsigned)n, threads, 0, stream>>>(a);
-        else sample_long_kernel<T, kList, kSampleThreads><<<(unsigned)n, threads, 0, stream>>>(a);
+        const int vecs = A / Row<T>::V;
+        const size_t smem = vecs <= kMaximaVecs ? (size_t)vecs * 4 : 0;
+        if (threads <= 64) {
+          sample_long_kernel<T, 512, 64><<<(unsigned)n, threads, smem, stream>>>(a);
+        } else {
+          auto kernel = sample_long_kernel<T, kList, kSampleThreads>;
+          if (smem > 24 * 1024)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaximaVecs * 4);
+          if (e != cudaSuccess) break;
+          kernel<<<(unsigned)n, threads, smem, stream>>>(a);
+        }
       }
     }
     e = cudaGetLastError();
