@@ -469,45 +469,65 @@ __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row
 
 template <int kSize> struct Shared {
   uint64_t slots[kSampleThreads / 32], list[kSize];
-  int counter;
+  int hit[kSize], hits, counter;
+  bool done;
+  uint32_t bounds[2];
 };
 
-// Draws from all of an unmasked row: the scores from the caches once more, and
-// the noise.  The row's weight is taken in 32 bits.
+// Draws from an unmasked row's actions from the rank key `last` on (0: all): the
+// scores from the caches once more, and the noise.  The kept weight is summed
+// in 32 bits.  Noisy scores are compared as they are defined, but with a
+// temperature the division is done only for vectors whose upper bound, from a
+// product with its reciprocal, could still win.
 template <typename T>
-__device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T>& r, const Filters& f, float top) {
+__device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T>& r, const Filters& f, float top,
+                              uint64_t last) {
   constexpr int V = Row<T>::V;
   const int tid = team.tid, n = team.n;
   const float* noise = r.noise ? r.noise + r.head : nullptr;
   const bool aligned = ((uintptr_t)noise & 15) == 0;
+  const float least = last ? key_score(last) : -FLT_MAX, per = 1.f / f.temperature;
+  const int last_index = last ? key_index(last) : GZ_POLICY_MAX_ACTIONS;
   float most = -INFINITY, z = 0.f;
-  int where = -1;  // vector of the best noisy score, or actions + the index of a score beside the vectors
-  auto scores = [&](int v, float* s, float* d) {
-    unpack<T>(r.vector(v), d);
+  int where = -1;
+  auto load = [&](int v, float* x, float* g) {  // scores, -inf where not kept
+    unpack<T>(r.vector(v), x);
 #pragma unroll
     for (int k = 0; k < V; k += 4) {
-      float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
       if (noise) {
         const float* p = noise + v * V + k;
-        g = aligned ? __ldg((const float4*)p) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+        q = aligned ? __ldg((const float4*)p) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float x = d[k + q];
-        d[k + q] = x > -INFINITY ? f.depth(fminf(x, FLT_MAX), top) : -INFINITY;
-        s[k + q] = d[k + q] + (&g.x)[q];
-      }
+      *(float4*)(g + k) = q;
     }
-  };
-#pragma unroll 2
-  for (int v = tid; v < r.vecs; v += n) {
-    float s[V], d[V];
-    scores(v, s, d);
-    float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      z += sm100::ex2_approx(d[k] * 1.44269504f);
-      m = fmaxf(m, s[k]);
+      const bool kept = x[k] > least || (x[k] == least && r.head + v * V + k <= last_index);
+      x[k] = kept ? fminf(x[k], FLT_MAX) : -INFINITY;
+    }
+  };
+  auto noisy = [&](float x, float g) { return x > -INFINITY ? f.depth(x, top) + g : -INFINITY; };
+#pragma unroll 2
+  for (int v = tid; v < r.vecs; v += n) {
+    float x[V], g[V], m = -INFINITY;
+    load(v, x, g);
+    if (f.min_p > 0.f) {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (x[k] > -INFINITY && expf(f.depth(x[k], top)) < f.min_p) x[k] = -INFINITY;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float d = (x[k] - top) * per;
+      z += sm100::ex2_approx(d * 1.44269504f);
+      // d is within 2^-22 |d| of the quotient
+      m = fmaxf(m, f.temperature == 1.f ? d + g[k] : fmaf(d, -0x1p-21f, d + g[k]));
+    }
+    if (f.temperature != 1.f && m + fabsf(m) * 0x1p-21f >= most) {
+      m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < V; ++k) m = fmaxf(m, noisy(x[k], g[k]));
     }
     if (m > most) {
       most = m;
@@ -516,17 +536,17 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
   }
   uint64_t best = 0;
   if (where >= 0) {
-    float s[V], d[V];
-    scores(where, s, d);
+    float x[V], g[V];
+    load(where, x, g);
 #pragma unroll
     for (int k = V - 1; k >= 0; --k)
-      if (s[k] == most) best = rank_key(most, r.head + where * V + k);
+      if (noisy(x[k], g[k]) == most && !(f.min_p > 0.f && expf(f.depth(x[k], top)) < f.min_p)) best = rank_key(most, r.head + where * V + k);
   }
   if (tid < r.ends) {
     const int j = r.end_index(tid);
-    const float x = to_f32(r.x[j]);
-    if (x > -INFINITY) {
-      const float d = f.depth(fminf(x, FLT_MAX), top), s = d + (r.noise ? r.noise[j] : 0.f);
+    const float x = fminf(to_f32(r.x[j]), FLT_MAX);
+    if (to_f32(r.x[j]) > -INFINITY && rank_key(x, j) >= last && !(f.min_p > 0.f && expf(f.depth(x, top)) < f.min_p)) {
+      const float d = f.depth(x, top), s = d + (r.noise ? r.noise[j] : 0.f);
       z += sm100::ex2_approx(d * 1.44269504f);
       const uint64_t key = rank_key(s >= -INFINITY ? s : -INFINITY, j);
       if (key > best) best = key;
@@ -534,11 +554,11 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
   }
   z = team.sum(z);
   best = team.max(best);
-  if (key_score(best) == -INFINITY || !best) {  // no score above -inf: the first visible action
+  if (!best || key_score(best) == -INFINITY) {  // no noisy score above -inf: the first of the kept actions
     best = 0;
-    each(r, tid, n, [&](int j, float) {
+    each(r, tid, n, [&](int j, float x) {
       const uint64_t key = rank_key(-INFINITY, j);
-      if (key > best) best = key;
+      if (rank_key(x, j) >= last && expf(f.depth(x, top)) >= f.min_p && key > best) best = key;
     });
     best = team.max(best);
   }
@@ -645,10 +665,12 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       }
       row_weight = (double)team.sum(z) * 0x1p44;
     }
-    // The largest number that enough threads' best scores reach: top_k of them;
-    // or so many that they weigh top_p of the row, or else half of them, which
-    // with what lies between them may still be enough.  One warp searches for
-    // it, over the scores' upper 16 bits, with weights in units of 2^-22.
+    // Bounds for the list: the largest number that enough threads' best scores
+    // reach, top_k of them, or so many that they weigh top_p of the row.  If
+    // all fall somewhat short of that (two of the best may be one thread's),
+    // 48 of them, then half of them, which with what lies between may still be
+    // enough.  One warp searches, over the scores' upper 16 bits, with weights
+    // in units of 2^-22.
     if (!by_count || f.top_k <= n) {
       uint32_t* scores = (uint32_t*)sh.list;
       scores[tid] = (uint32_t)(mine >> 18);
@@ -675,33 +697,37 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
           }
         least = __reduce_min_sync(~0u, least);
         most = __reduce_max_sync(~0u, most);
-        uint32_t goal = f.top_k;
-        if (!by_count) {
-          const double g = f.top_p * row_weight * 0x1p-22 * 1.00001 + 1;
-          goal = g < 0x1p31 ? (uint32_t)g : ~0u;
-          const uint32_t all = above(1);
-          if (all < goal / 2) {
-            goal = ~0u;  // hopeless
-          } else if (all < goal) {
-            goal = n / 2;
-#pragma unroll
-            for (int i = 0; i < kSampleThreads / 32; ++i) weight[i] = 1;
-          }
-        }
         // the bits that all scores share need no search
         const int first = 31 - __clz(least ^ most | 1);
-        uint32_t reach = above(1) >= goal ? most & ~((2u << first) - 1) : 0;
-        if (reach)
+        auto reach = [&](uint32_t goal) {
+          uint32_t bound = above(1) >= goal ? most & ~((2u << first) - 1) : 0;
+          if (bound)
 #pragma unroll 1
-          for (int bit = first; bit >= kReachBit; --bit)
-            if (above(reach | 1u << bit) >= goal) reach |= 1u << bit;
-        if (tid == 0) *(uint32_t*)sh.slots = reach;
+            for (int bit = first; bit >= kReachBit; --bit)
+              if (above(bound | 1u << bit) >= goal) bound |= 1u << bit;
+          return bound;
+        };
+        uint32_t bounds[2] = {0, 0};
+        if (by_count) {
+          bounds[0] = reach(f.top_k);
+        } else {
+          const double g = f.top_p * row_weight * 0x1p-22 * 1.00001 + 1;
+          const uint32_t goal = g < 0x1p31 ? (uint32_t)g : 0x7fffffffu, all = above(1);
+          if (all >= goal) {
+            bounds[0] = reach(goal);
+          } else if (all >= goal / 2) {
+#pragma unroll
+            for (int i = 0; i < kSampleThreads / 32; ++i) weight[i] = 1;
+            bounds[0] = reach(min(48, n / 2));
+            if (n / 2 > 48) bounds[1] = reach(n / 2);
+          }
+        }
+        if (tid == 0) sh.bounds[0] = bounds[0], sh.bounds[1] = bounds[1];
       }
       __syncthreads();
-      const uint32_t reach = *(uint32_t*)sh.slots;
-      if (reach) {
-        const float from = key_value(reach);
-        if (tid == 0) sh.counter = 0;
+      for (int attempt = 0; attempt < 2 && sh.bounds[attempt]; ++attempt) {
+        const float from = key_value(sh.bounds[attempt]);
+        if (tid == 0) sh.counter = sh.hits = 0;
         __syncthreads();
         auto take = [&](int j, float x) {
           if (x >= from) {
@@ -720,10 +746,20 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
             for (int k = 0; k < V; ++k)
               if (x[k] == x[k]) take(r.head + v * V + k, fminf(x[k], FLT_MAX));
           };
-          if (maxima) {  // each thread the vectors that it has read
-#pragma unroll 4
+          if (maxima) {  // each thread's own vectors' maxima; then their scores, all at once
+#pragma unroll 8
             for (int v = tid; v < r.vecs; v += n)
-              if (maxima[v] >= from) take_vector(v, r.vector(v));
+              if (maxima[v] >= from) {
+                const int at = atomicAdd(&sh.hits, 1);
+                if (at < kSize) sh.hit[at] = v;
+              }
+            __syncthreads();
+            const int hits = sh.hits;
+            if (hits > kSize) {
+              __syncthreads();  // all have seen it
+              continue;
+            }
+            for (int h = tid; h < hits; h += n) take_vector(sh.hit[h], r.vector(sh.hit[h]));
           } else {
             constexpr int kAhead = 4;
             for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
@@ -750,10 +786,10 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
               x[i] = key_score(key);
             }
             const bool done = draw_from_few(a, row, r, f, j, x, row_weight, *(FewShared*)(sh.list + kFew));
-            if (tid == 0) sh.counter = done;
+            if (tid == 0) sh.done = done;
           }
           __syncthreads();
-          if (sh.counter) return;
+          if (sh.done) return;
         } else if (m <= kSize && draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
       }
     }
@@ -774,17 +810,15 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       if (cut > last) last = cut;
     }
   }
-  if (kMasked || last || f.min_p > 0.f) {
-    const float score = last ? key_score(last) : -INFINITY, floor = f.min_p > 0.f ? logf(f.min_p) - 0.01f : -INFINITY;
+  if (kMasked) {
     Draw d;
     each(r, tid, n, [&](int j, float x) {
-      if (x < score || (x == score && j > key_index(last)) || (x - top) < floor * f.temperature * 1.01f) return;
-      d.add(f, top, x, j, r.noise);
+      if (rank_key(x, j) >= last) d.add(f, top, x, j, r.noise);
     });
     d.finish(a, row, team, r, f, top);
-    return;
+  } else {
+    draw_from_all(a, row, team, r, f, top, last);
   }
-  draw_from_all(a, row, team, r, f, top);
 }
 
 // A call of its own, so that rows that fit the list do not pay for its registers.
