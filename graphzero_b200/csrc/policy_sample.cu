@@ -45,8 +45,11 @@ constexpr int kReachBit = 16;       // lowest bit of a score that the search for
 constexpr int kMaximaVecs = 24576;  // vectors of a row whose maxima are kept (96 KB: two blocks fit an SM)
 constexpr int64_t kRowsPerLaunch = 1 << 28;
 
-// exp(d) in units of 2^-44 (d <= 0): 2^18 actions sum below 2^63.
-__device__ __forceinline__ uint64_t fixed_weight(float e) { return __float2ull_rd(e * 0x1p44f); }
+// e = exp(d), 0 .. 1, in units of 2^-44, cut off: 2^18 actions sum below 2^63.
+__device__ __forceinline__ uint64_t fixed_weight(float e) {
+  const uint32_t b = __float_as_uint(e);
+  return (uint64_t)(b & 0x7fffffu | 0x800000u) << 21 >> min(63u, 127 - (b >> 23));  // 24 bits, shifted by the exponent
+}
 
 // Rank order as one number: higher scores first, at equal scores lower indices.
 __device__ __forceinline__ uint64_t rank_key(float x, int j) {
@@ -332,6 +335,7 @@ __device__ __forceinline__ bool draw_from_few(const SampleArgs& a, int64_t row, 
       const uint32_t some = __ballot_sync(~0u, key[i] != 0);
       if (some) full = 32 * i + 32 - __clz(some);
     }
+#pragma unroll 4
     for (int q = 0; q < full; ++q) {
       const uint64_t k = sh.key[q], w = sh.weight[q];
 #pragma unroll
@@ -417,7 +421,7 @@ __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row
   __shared__ int found;
   constexpr int kBins = kSize;
   uint32_t *low = (uint32_t*)memory, *high = low + kBins;
-  const float scale = kBins / (31.f * f.temperature);
+  const float scale = kBins / (31.f * f.temperature), per_score = 1.44269504f / f.temperature;
   auto bin = [&](float x) { return min(kBins - 1, (int)((top - x) * scale)); };  // falls as x rises, weakly
   team.sync();
   for (int i = team.tid; i < kBins; i += team.n) low[i] = high[i] = 0;
@@ -425,7 +429,8 @@ __device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row
   team.sync();
   each(r, team.tid, team.n, [&](int, float x) {
     if (x < from) return;
-    const uint64_t w = kWeights ? fixed_weight(expf(f.depth(x, top))) : 1;
+    // (the bins' weights by the fast exponential; the boundary bin's by the list's)
+    const uint64_t w = kWeights ? fixed_weight(sm100::ex2_approx((x - top) * per_score)) : 1;
     if (!w) return;
     // in two halves, for only 32-bit adds are done in shared memory at once
     const int b = bin(x);
