@@ -476,7 +476,7 @@ template <int kSize> struct Shared {
   uint64_t slots[kSampleThreads / 32], list[kSize];
   int hit[kSize], hits, counter;
   bool done;
-  uint32_t bounds[2];
+  uint32_t bound, sums[3];
 };
 
 // Draws from an unmasked row's actions from the rank key `last` on (0: all): the
@@ -574,6 +574,72 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
 }
 
 // A row whose visible actions do not all fit the list.
+// Draws by top_p from a list of m actions, more than kFew, without sorting it.
+// Weights in units of 2^-22, cut off, are summed above a score that a search
+// over its bits raises as far as the goal is surely reached; what is left has
+// few actions too many, and those go one by one, the least first, by exact
+// weights.  False: not done (the list or the cut weights do not reach the goal,
+// or too many actions are at the boundary).
+template <typename T, int kSize>
+__device__ bool draw_by_weight(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T>& r, const Filters& f,
+                               Shared<kSize>& sh, int m, float from, float top, double row_weight) {
+  const int tid = team.tid, n = team.n;
+  const double goal = f.top_p * row_weight, cut = goal * 0x1p-22 + 1;
+  if (cut >= 0x1p31) return false;
+  const uint32_t goal22 = (uint32_t)cut + 1;
+  uint32_t* weight = (uint32_t*)sh.hit;
+  for (int i = tid; i < m; i += n) weight[i] = (uint32_t)(fixed_weight(expf(f.depth(key_score(sh.list[i]), top))) >> 22);
+  if (tid < 3) sh.sums[tid] = 0;
+  team.sync();
+  int round = 0;
+  auto above = [&](uint32_t score) {  // weight of the scores from this one on
+    uint32_t c = 0;
+    for (int i = tid; i < m; i += n)
+      if ((uint32_t)(sh.list[i] >> 18) >= score) c += weight[i];
+    c = __reduce_add_sync(~0u, c);
+    uint32_t* sum = &sh.sums[round % 3];
+    if (tid % 32 == 0 && c) atomicAdd(sum, c);
+    if (tid == 0) sh.sums[(round + 1) % 3] = 0;
+    ++round;
+    __syncthreads();
+    return *sum;
+  };
+  // (the sum cannot pass 2^32: it is at most the row's weight, below 2^31 / top_p)
+  const uint32_t low = order_key(from), high = order_key(top);
+  if (above(low) < goal22) return false;
+  const int first = 31 - __clz(low ^ high | 1);
+  uint32_t score = high & ~((2u << first) - 1);
+#pragma unroll 1
+  for (int bit = first; bit >= (sizeof(T) == 2 ? 13 : 6); --bit)
+    if (above(score | 1u << bit) >= goal22) score |= 1u << bit;
+  // the list's actions from `score` on
+  uint64_t sum = 0;
+  for (int i = tid; i < m; i += n)
+    if ((uint32_t)(sh.list[i] >> 18) >= score) sum += fixed_weight(expf(f.depth(key_score(sh.list[i]), top)));
+  sum = team.sum(sum);
+  uint64_t least = 0;  // the last key that is dropped
+  for (int round = 0;; ++round) {
+    uint64_t key = ~0ull;
+    for (int i = tid; i < m; i += n) {
+      const uint64_t k = sh.list[i];
+      if ((uint32_t)(k >> 18) >= score && k > least && k < key) key = k;
+    }
+    key = team.reduce(key, [](uint64_t x, uint64_t y) { return x < y ? x : y; });
+    const uint64_t w = fixed_weight(expf(f.depth(key_score(key), top)));
+    if ((double)(sum - w) < goal) break;
+    if (round == 16) return false;
+    sum -= w;
+    least = key;
+  }
+  Draw d;
+  for (int i = tid; i < m; i += n) {
+    const uint64_t k = sh.list[i];
+    if ((uint32_t)(k >> 18) >= score && k > least) d.add(f, top, key_score(k), key_index(k), r.noise);
+  }
+  d.finish(a, row, team, r, f, top);
+  return true;
+}
+
 // maxima: a float for every vector of the row, or null.
 template <typename T, bool kMasked, int kSize>
 __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh, float* maxima) {
@@ -670,68 +736,53 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       }
       row_weight = (double)team.sum(z) * 0x1p44;
     }
-    // Bounds for the list: the largest number that enough threads' best scores
-    // reach, top_k of them, or so many that they weigh top_p of the row.  If
-    // all fall somewhat short of that (two of the best may be one thread's),
-    // 48 of them, then half of them, which with what lies between may still be
-    // enough.  One warp searches, over the scores' upper 16 bits, with weights
-    // in units of 2^-22.
-    if (!by_count || f.top_k <= n) {
+    // Bounds for the list.  For top_k the largest number that top_k threads' best
+    // scores reach; one warp searches for it, over the scores' upper 16 bits.
+    // For top_p the scores whose weight is 1/16, then 1/512 of what top_p leaves
+    // out: no more than 16 / (1 - top_p) actions reach the first, and what lies
+    // below it is often little.
+    float bounds[2] = {-INFINITY, -INFINITY};
+    if (!by_count) {
+      const float out = (float)((1.0 - f.top_p) * row_weight * 0x1p-44);
+      bounds[0] = top + fminf(logf(out * (1.f / 16)), 0.f) * f.temperature;
+      bounds[1] = top + fminf(logf(out * (1.f / 512)), 0.f) * f.temperature;
+    } else if (f.top_k <= n) {
       uint32_t* scores = (uint32_t*)sh.list;
       scores[tid] = (uint32_t)(mine >> 18);
       __syncthreads();
       if (tid < 32) {
-        uint32_t score[kSampleThreads / 32], weight[kSampleThreads / 32];
+        uint32_t score[kSampleThreads / 32], least = ~0u, most = 0;
 #pragma unroll
         for (int i = 0; i < kSampleThreads / 32; ++i) {
           score[i] = i < n / 32 ? scores[tid + 32 * i] : 0;
-          weight[i] = by_count ? 1 : score[i] ? (uint32_t)(expf(f.depth(key_value(score[i]), top)) * 0x1p22f) : 0;
-        }
-        auto above = [&](uint32_t mid) {
-          uint32_t c = 0;
-#pragma unroll
-          for (int i = 0; i < kSampleThreads / 32; ++i) c += score[i] >= mid ? weight[i] : 0;
-          return __reduce_add_sync(~0u, c);
-        };
-        uint32_t least = ~0u, most = 0;
-#pragma unroll
-        for (int i = 0; i < kSampleThreads / 32; ++i)
           if (score[i]) {
             least = min(least, score[i]);
             most = max(most, score[i]);
           }
+        }
+        auto above = [&](uint32_t mid) {
+          int c = 0;
+#pragma unroll
+          for (int i = 0; i < kSampleThreads / 32; ++i) c += score[i] >= mid;
+          return __reduce_add_sync(~0u, c);
+        };
         least = __reduce_min_sync(~0u, least);
         most = __reduce_max_sync(~0u, most);
         // the bits that all scores share need no search
         const int first = 31 - __clz(least ^ most | 1);
-        auto reach = [&](uint32_t goal) {
-          uint32_t bound = above(1) >= goal ? most & ~((2u << first) - 1) : 0;
-          if (bound)
+        uint32_t bound = above(1) >= f.top_k ? most & ~((2u << first) - 1) : 0;
+        if (bound)
 #pragma unroll 1
-            for (int bit = first; bit >= kReachBit; --bit)
-              if (above(bound | 1u << bit) >= goal) bound |= 1u << bit;
-          return bound;
-        };
-        uint32_t bounds[2] = {0, 0};
-        if (by_count) {
-          bounds[0] = reach(f.top_k);
-        } else {
-          const double g = f.top_p * row_weight * 0x1p-22 * 1.00001 + 1;
-          const uint32_t goal = g < 0x1p31 ? (uint32_t)g : 0x7fffffffu, all = above(1);
-          if (all >= goal) {
-            bounds[0] = reach(goal);
-          } else if (all >= goal / 2) {
-#pragma unroll
-            for (int i = 0; i < kSampleThreads / 32; ++i) weight[i] = 1;
-            bounds[0] = reach(min(48, n / 2));
-            if (n / 2 > 48) bounds[1] = reach(n / 2);
-          }
-        }
-        if (tid == 0) sh.bounds[0] = bounds[0], sh.bounds[1] = bounds[1];
+          for (int bit = first; bit >= kReachBit; --bit)
+            if (above(bound | 1u << bit) >= f.top_k) bound |= 1u << bit;
+        if (tid == 0) sh.bound = bound;
       }
       __syncthreads();
-      for (int attempt = 0; attempt < 2 && sh.bounds[attempt]; ++attempt) {
-        const float from = key_value(sh.bounds[attempt]);
+      if (sh.bound) bounds[0] = key_value(sh.bound);
+    }
+    {
+      for (int attempt = 0; attempt < 2 && bounds[attempt] > -INFINITY; ++attempt) {
+        const float from = bounds[attempt];
         if (tid == 0) sh.counter = sh.hits = 0;
         __syncthreads();
         auto take = [&](int j, float x) {
@@ -795,7 +846,10 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
           }
           __syncthreads();
           if (sh.done) return;
-        } else if (m <= kSize && draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
+        } else if (m <= kSize) {
+          if (!by_count && draw_by_weight(a, row, team, r, f, sh, m, from, top, row_weight)) return;
+          if (draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
+        }
       }
     }
     if (by_count) last = last_by_bins<false, kSize>(team, r, f, top, (double)f.top_k, -INFINITY, sh.list, &sh.counter);
