@@ -81,6 +81,30 @@ def test_sample_filters(cuda, a, share, kw):
     check_sample(x, noise, None if share is None else legal(n, a, share, 13), **kw)
 
 
+@pytest.mark.parametrize("spread", [0.05, 0.5, 1.5])
+@pytest.mark.parametrize("a", [65, 100, 256, 500, 1100, 2048, 2049, 5000, 9001, 40000])
+def test_sample_flat_rows(cuda, a, spread):
+    """Kept shares from a few actions to nearly all, in lists of every length and beyond them."""
+    n = 4 if a <= 9001 else 2
+    for dtype in (torch.float32, torch.bfloat16):
+        x, noise = rows_of(n, a, a, dtype, spread=spread), ref.gumbel((n, a), a + 2)
+        for kw in (dict(top_p=0.02), dict(top_p=0.3), dict(top_p=0.9), dict(top_p=0.9, temperature=0.7), dict(top_k=a // 3),
+                   dict(top_k=a - 1, top_p=0.95), dict(top_k=40, top_p=0.5), dict(top_p=0.8, min_p=0.2)):
+            check_sample(x, noise, **kw)
+
+
+@pytest.mark.parametrize("a", [400, 4672, 5121, 40000])
+def test_sample_masks_of_every_density(cuda, a):
+    """From none to all of a block's rows with more visible actions than a list holds."""
+    n = 9
+    x, noise = rows_of(n, a, 3, torch.float16), ref.gumbel((n, a), 4)
+    share = torch.tensor([0.0, 0.001, 0.02, 0.05, 0.2, 0.5, 0.9, 1.0, 0.01])
+    g = torch.Generator().manual_seed(5)
+    mask = (torch.rand(n, a, generator=g) < share[:, None]).to(torch.uint8) * 255
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=70), dict(top_k=300, top_p=0.7, min_p=0.01), dict(temperature=0.0)):
+        check_sample(x, noise, mask, **kw)
+
+
 def test_sample_many_rows_per_row_settings(cuda):
     n, a = 700, 129
     g = torch.Generator().manual_seed(5)
