@@ -76,6 +76,22 @@ template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint4 raw, flo
   }
 }
 
+// Visibility of V actions, a bit each.
+template <int V> __device__ __forceinline__ uint32_t visible_bits(const uint8_t* mask, bool aligned) {
+  uint32_t bits = 0;
+  if (aligned) {
+    uint32_t w[V / 4];
+    if (V == 4) w[0] = __ldg((const uint32_t*)mask);
+    else *(uint2*)w = __ldg((const uint2*)mask);
+#pragma unroll
+    for (int k = 0; k < V; ++k) bits |= ((w[k / 4] >> (8 * (k % 4)) & 0xff) != 0) << k;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) bits |= (__ldg(mask + k) != 0) << k;
+  }
+  return bits;
+}
+
 // Maximum of a vector's visible scores and m.
 template <bool kMasked, typename T>
 __device__ __forceinline__ float max_vector(float m, uint4 raw, uint32_t bits) {

@@ -80,22 +80,6 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 __device__ __forceinline__ void end_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-// Visibility of V actions, a bit each.
-template <int V> __device__ __forceinline__ uint32_t visible_bits(const uint8_t* mask, bool aligned) {
-  uint32_t bits = 0;
-  if (aligned) {
-    uint32_t w[V / 4];
-    if (V == 4) w[0] = __ldg((const uint32_t*)mask);
-    else *(uint2*)w = __ldg((const uint2*)mask);
-#pragma unroll
-    for (int k = 0; k < V; ++k) bits |= ((w[k / 4] >> (8 * (k % 4)) & 0xff) != 0) << k;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) bits |= (__ldg(mask + k) != 0) << k;
-  }
-  return bits;
-}
-
 template <int V> __device__ __forceinline__ void load_floats(const float* p, bool aligned, float* x) {
 #pragma unroll
   for (int k = 0; k < V; k += 4)

@@ -35,7 +35,6 @@ struct SampleArgs {
   int32_t* action;
   float* logp;
   int64_t first_row, end_row;  // of this launch
-  int row_warps;               // warps a masked row gets
 };
 
 constexpr int kList = 2048;         // keys a block's list holds
@@ -104,12 +103,14 @@ template <bool kWarp> struct Team {
   }
 };
 
-template <typename T> struct Row {
+// kMask: vectors are read through the mask.
+template <typename T, bool kMask> struct Row {
   static constexpr int V = 16 / (int)sizeof(T);
   const T* x;
   const uint8_t* mask;
   const float* noise;
   int actions, head, vecs, ends;  // scores before the first 16-byte boundary, vectors, scores beside them
+  bool mask_aligned;
 
   __device__ Row(const SampleArgs& a, int64_t row) {
     actions = a.rows.actions;
@@ -119,15 +120,32 @@ template <typename T> struct Row {
     head = min(actions, (int)(-(uintptr_t)x & 15) / (int)sizeof(T));
     vecs = (actions - head) / V;
     ends = actions - vecs * V;
+    mask_aligned = (((uintptr_t)mask + head) & (V - 1)) == 0;
   }
   __device__ int end_index(int i) const { return i < head ? i : actions - ends + i; }
-  __device__ uint4 vector(int v) const { return __ldg((const uint4*)(x + head) + v); }
+  __device__ float end_score(int i) const {
+    const int j = end_index(i);
+    return kMask && !mask[j] ? -INFINITY : to_f32(x[j]);
+  }
+  // A vector's scores, -inf where masked.
+  __device__ __forceinline__ uint4 vector(int v) const {
+    const uint4* p = (const uint4*)(x + head) + v;
+    if (!kMask) return __ldg(p);
+    const uint32_t bits = visible_bits<V>(mask + head + v * V, mask_aligned);
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (bits) raw = __ldg(p);
+    T* e = (T*)&raw;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (!(bits >> k & 1)) e[k] = from_f32<T>(-INFINITY);
+    return raw;
+  }
 };
 
 // f(first, bits) for this thread's share of a mask, sixteen bytes at a time and
 // the bytes beside the whole sixteens one by one: bits of visible actions from
 // `first` on, none of them 0.  Needs at least 30 threads.
-template <int kAhead, typename T, typename F> __device__ __forceinline__ void each_visible(const Row<T>& r, int tid, int n, F f) {
+template <int kAhead, typename T, typename F, bool kMask> __device__ __forceinline__ void each_visible(const Row<T, kMask>& r, int tid, int n, F f) {
   const int head = min(r.actions, (int)(-(uintptr_t)r.mask & 15));
   const int groups = (r.actions - head) / 16, ends = r.actions - groups * 16;
   const int ej = tid < head ? tid : r.actions - ends + tid;
@@ -152,25 +170,17 @@ template <int kAhead, typename T, typename F> __device__ __forceinline__ void ea
 }
 
 // f(j, score) for this thread's share of the visible actions.
-template <typename T, typename F> __device__ __forceinline__ void each(const Row<T>& r, int tid, int n, F f) {
+template <typename T, typename F, bool kMask> __device__ __forceinline__ void each(const Row<T, kMask>& r, int tid, int n, F f) {
   auto one = [&](int j, float v) {
     if (v > -INFINITY) f(j, fminf(v, FLT_MAX));  // a NaN counts as -inf
   };
-  if (r.mask) {
-    each_visible<2>(r, tid, n, [&](int first, uint32_t bits) {
-      for (; bits; bits &= bits - 1) {
-        const int j = first + __ffs(bits) - 1;
-        one(j, to_f32(r.x[j]));
-      }
-    });
-  } else {
-    if (tid < r.ends) one(r.end_index(tid), to_f32(r.x[r.end_index(tid)]));
-    for (int v = tid; v < r.vecs; v += n) {
-      float x[Row<T>::V];
-      unpack<T>(r.vector(v), x);
+  if (tid < r.ends) one(r.end_index(tid), r.end_score(tid));
+  for (int v = tid; v < r.vecs; v += n) {
+    constexpr int V = 16 / (int)sizeof(T);
+    float x[V];
+    unpack<T>(r.vector(v), x);
 #pragma unroll
-      for (int k = 0; k < Row<T>::V; ++k) one(r.head + v * Row<T>::V + k, x[k]);
-    }
+    for (int k = 0; k < V; ++k) one(r.head + v * V + k, x[k]);
   }
 }
 
@@ -181,6 +191,7 @@ struct Filters {
 
   __device__ Filters(const gz_sample_config& c, int64_t row) {
     temperature = fminf(c.d_temperature ? c.d_temperature[row] : c.temperature, FLT_MAX);
+    if (temperature > 0.f) temperature = fmaxf(temperature, 1e-30f);  // its reciprocal stays finite
     top_p = c.d_top_p ? c.d_top_p[row] : c.top_p;
     min_p = fminf(c.d_min_p ? c.d_min_p[row] : c.min_p, 1.f);
     top_k = c.d_top_k ? c.d_top_k[row] : c.top_k;
@@ -205,8 +216,8 @@ struct Draw {
     const uint64_t key = rank_key(s >= -INFINITY ? s : -INFINITY, j);
     if (key > best) best = key;
   }
-  template <typename T, bool kWarp>
-  __device__ void finish(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T>& r, const Filters& f, float top) {
+  template <typename T, bool kWarp, bool kMask>
+  __device__ void finish(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T, kMask>& r, const Filters& f, float top) {
     weight = team.sum(weight);
     best = team.max(best);
     if (team.tid == 0) {
@@ -259,8 +270,8 @@ __device__ int keys_before(const Team<kWarp>& team, const uint64_t* keys, int m,
 // in memory, of which `count` are not 0.  row_weight < 0: the list is the whole
 // row or top_k's; else the row's weight, and false comes back if the list does
 // not reach top_p's share of it.
-template <typename T, bool kWarp>
-__device__ bool draw_from_list(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T>& r, const Filters& f,
+template <typename T, bool kWarp, bool kMask>
+__device__ bool draw_from_list(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T, kMask>& r, const Filters& f,
                                uint64_t* keys, int size, int count, float top, double row_weight) {
   if ((f.top_k > 0 && f.top_k < count) || f.top_p < 1.f) {
     sort_keys(team, keys, size);
@@ -288,8 +299,8 @@ constexpr int kFew = 64, kMine = kFew / 32;
 struct FewShared {
   uint64_t key[kFew], weight[kFew];
 };
-template <typename T>
-__device__ __forceinline__ bool draw_from_few(const SampleArgs& a, int64_t row, const Row<T>& r, const Filters& f, const int* j,
+template <typename T, bool kMask>
+__device__ __forceinline__ bool draw_from_few(const SampleArgs& a, int64_t row, const Row<T, kMask>& r, const Filters& f, const int* j,
                                               const float* x, double row_weight, FewShared& sh) {
   const Team<true> team{nullptr, (int)threadIdx.x % 32, 32};
   float noise[kMine], d[kMine], e[kMine];
@@ -382,7 +393,7 @@ template <typename T> __global__ void __launch_bounds__(128) sample_warp_kernel(
   const int64_t row = a.first_row + (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= a.end_row) return;
   const int lane = threadIdx.x % 32;
-  const Row<T> r(a, row);
+  const Row<T, false> r(a, row);
   const Filters f(a.cfg, row);
   int j[kMine];
   float x[kMine];
@@ -397,8 +408,8 @@ template <typename T> __global__ void __launch_bounds__(128) sample_warp_kernel(
 
 // The rank key of the last kept action: the largest with at least `goal` (a
 // count, or a weight) at or above it.
-template <bool kWeights, typename T>
-__device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal) {
+template <bool kWeights, typename T, bool kMask>
+__device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, const Row<T, kMask>& r, const Filters& f, float top, double goal) {
   uint64_t last = 0;
   for (int bit = 49; bit >= 0; --bit) {
     const uint64_t mid = last | 1ull << bit;
@@ -411,17 +422,17 @@ __device__ __noinline__ uint64_t last_by_bisection(const Team<false>& team, cons
   return last;
 }
 
-// The same through a histogram, in the list's memory, over the 31 temperatures
-// below the best score (what lies deeper is found by bisection if need be).
+// The same through a histogram, in the list's memory, over `span` below the best
+// score (what lies deeper is found by bisection if need be).
 // Scores below `from` are known not to be kept.
-template <bool kWeights, int kSize, typename T>
-__device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row<T>& r, const Filters& f, float top, double goal,
-                                              float from, uint64_t* memory, int* counter) {
+template <bool kWeights, int kSize, typename T, bool kMask>
+__device__ __noinline__ uint64_t last_by_bins(const Team<false>& team, const Row<T, kMask>& r, const Filters& f, float top, double goal,
+                                              float from, float span, uint64_t* memory, int* counter) {
   __shared__ uint64_t above;
   __shared__ int found;
   constexpr int kBins = kSize;
   uint32_t *low = (uint32_t*)memory, *high = low + kBins;
-  const float scale = kBins / (31.f * f.temperature), per_score = 1.44269504f / f.temperature;
+  const float scale = kBins / span, per_score = 1.44269504f / f.temperature;
   auto bin = [&](float x) { return min(kBins - 1, (int)((top - x) * scale)); };  // falls as x rises, weakly
   team.sync();
   for (int i = team.tid; i < kBins; i += team.n) low[i] = high[i] = 0;
@@ -482,19 +493,20 @@ template <int kSize> struct Shared {
 
 // Draws from an unmasked row's actions from the rank key `last` on (0: all): the
 // scores from the caches once more, and the noise.  The kept weight is summed
-// in 32 bits.  Noisy scores are compared as they are defined, but with a
+// in 32 bits (under a mask in whole numbers).  Noisy scores are compared as they are defined, but with a
 // temperature the division is done only for vectors whose upper bound, from a
 // product with its reciprocal, could still win.
-template <typename T>
-__device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T>& r, const Filters& f, float top,
+template <typename T, bool kMask>
+__device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T, kMask>& r, const Filters& f, float top,
                               uint64_t last) {
-  constexpr int V = Row<T>::V;
+  constexpr int V = (16 / (int)sizeof(T));
   const int tid = team.tid, n = team.n;
   const float* noise = r.noise ? r.noise + r.head : nullptr;
   const bool aligned = ((uintptr_t)noise & 15) == 0;
   const float least = last ? key_score(last) : -FLT_MAX, per = 1.f / f.temperature;
   const int last_index = last ? key_index(last) : GZ_POLICY_MAX_ACTIONS;
   float most = -INFINITY, z = 0.f;
+  uint64_t weight = 0;  // the same in whole numbers, under a mask: whatever the mask's alignment to the scores
   int where = -1;
   auto load = [&](int v, float* x, float* g) {  // scores, -inf where not kept
     unpack<T>(r.vector(v), x);
@@ -526,7 +538,9 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const float d = (x[k] - top) * per;
-      z += sm100::ex2_approx(d * 1.44269504f);
+      const float e = sm100::ex2_approx(d * 1.44269504f);
+      if (kMask) weight += fixed_weight(e);
+      else z += e;
       // d is within 2^-22 |d| of the quotient
       m = fmaxf(m, f.temperature == 1.f ? d + g[k] : fmaf(d, -0x1p-21f, d + g[k]));
     }
@@ -550,15 +564,17 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
   }
   if (tid < r.ends) {
     const int j = r.end_index(tid);
-    const float x = fminf(to_f32(r.x[j]), FLT_MAX);
-    if (to_f32(r.x[j]) > -INFINITY && rank_key(x, j) >= last && !(f.min_p > 0.f && expf(f.depth(x, top)) < f.min_p)) {
+    const float x = fminf(r.end_score(tid), FLT_MAX);
+    if (r.end_score(tid) > -INFINITY && rank_key(x, j) >= last && !(f.min_p > 0.f && expf(f.depth(x, top)) < f.min_p)) {
       const float d = f.depth(x, top), s = d + (r.noise ? r.noise[j] : 0.f);
-      z += sm100::ex2_approx(d * 1.44269504f);
+      const float e = sm100::ex2_approx((x - top) * per * 1.44269504f);
+      if (kMask) weight += fixed_weight(e);
+      else z += e;
       const uint64_t key = rank_key(s >= -INFINITY ? s : -INFINITY, j);
       if (key > best) best = key;
     }
   }
-  z = team.sum(z);
+  z = kMask ? (float)((double)team.sum(weight) * 0x1p-44) : team.sum(z);
   best = team.max(best);
   if (!best || key_score(best) == -INFINITY) {  // no noisy score above -inf: the first of the kept actions
     best = 0;
@@ -579,8 +595,8 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
 // a key's rank and the weight before it come from comparing it with all others.
 // row_weight and the answer as in draw_from_list.
 constexpr int kRanked = 256;
-template <typename T, int kSize>
-__device__ bool draw_by_rank(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T>& r, const Filters& f,
+template <typename T, int kSize, bool kMask>
+__device__ bool draw_by_rank(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T, kMask>& r, const Filters& f,
                              Shared<kSize>& sh, int m, float top, double row_weight) {
   static_assert(2 * kRanked <= kSize, "keys, and the weights before them, lie in the list");
   uint64_t *key = sh.list, *before = sh.list + kRanked, *weight = (uint64_t*)sh.hit;
@@ -622,8 +638,8 @@ __device__ bool draw_by_rank(const SampleArgs& a, int64_t row, const Team<false>
 // few actions too many, and those go one by one, the least first, by exact
 // weights.  False: not done (the list or the cut weights do not reach the goal,
 // or too many actions are at the boundary).
-template <typename T, int kSize, bool kWarp>
-__device__ bool draw_by_weight(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T>& r, const Filters& f,
+template <typename T, int kSize, bool kWarp, bool kMask>
+__device__ bool draw_by_weight(const SampleArgs& a, int64_t row, const Team<kWarp>& team, const Row<T, kMask>& r, const Filters& f,
                                Shared<kSize>& sh, int m, float from, float top, double row_weight) {
   const int tid = team.tid, n = team.n;
   const double goal = f.top_p * row_weight, cut = goal * 0x1p-22 + 1;
@@ -683,13 +699,14 @@ __device__ bool draw_by_weight(const SampleArgs& a, int64_t row, const Team<kWar
   return true;
 }
 
-// maxima: a float for every vector of the row, or null.
-template <typename T, bool kMasked, int kSize>
+// maxima: a float for every vector of the row, or null.  kMask: it is read
+// through its mask.
+template <typename T, bool kMask, int kSize>
 __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh, float* maxima) {
-  constexpr int V = Row<T>::V;
+  constexpr int V = (16 / (int)sizeof(T));
   const int tid = threadIdx.x, n = blockDim.x;
   const Team<false> team{sh.slots, tid, n};
-  const Row<T> r(a, row);
+  const Row<T, kMask> r(a, row);
   const Filters f(a.cfg, row);
   const bool by_count = f.top_k > 0 && f.top_k < r.actions, by_weight = f.top_p < 1.f;
   const bool row_weighs = by_weight && !by_count && !f.greedy;
@@ -700,65 +717,58 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
   uint64_t best = 0;
   float z = 0.f, z_base = -INFINITY;
   bool z_fine = false;
-  if (kMasked) {
-    each(r, tid, n, [&](int j, float x) {
-      const uint64_t key = rank_key(x, j);
-      if (key > best) best = key;
-    });
-  } else {
-    float most = -INFINITY, c = 0.f;
-    int where = -1;
-    float2 sum = {0.f, 0.f};
-    constexpr int kAhead = 4;
-    for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
-      uint4 raw[kAhead];
+  float most = -INFINITY, base = 0.f;
+  int where = -1;
+  float2 sum = {0.f, 0.f};
+  constexpr int kAhead = 4;
+  for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
+    uint4 raw[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (v0 + i * n < r.vecs) raw[i] = r.vector(v0 + i * n);
+    for (int i = 0; i < kAhead; ++i)
+      if (v0 + i * n < r.vecs) raw[i] = r.vector(v0 + i * n);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (v0 + i * n >= r.vecs) continue;
-        const float m = fminf(max_vector<false, T>(-INFINITY, raw[i], 0), FLT_MAX);
-        if (maxima) maxima[v0 + i * n] = m;
-        if (m > most) {
-          most = m;
-          where = v0 + i * n;
+    for (int i = 0; i < kAhead; ++i) {
+      if (v0 + i * n >= r.vecs) continue;
+      const float m = fminf(max_vector<false, T>(-INFINITY, raw[i], 0), FLT_MAX);
+      if (maxima) maxima[v0 + i * n] = m;
+      if (m > most) {
+        most = m;
+        where = v0 + i * n;
+      }
+      if (row_weighs) {
+        if (z_base == -INFINITY) {
+          z_base = m;
+          base = m == -INFINITY ? 0.f : m;
         }
-        if (row_weighs) {
-          if (z_base == -INFINITY) {
-            z_base = m;
-            c = m == -INFINITY ? 0.f : -m * per_score;
-          }
-          float x[V];
-          unpack<T>(raw[i], x);
+        float x[V];
+        unpack<T>(raw[i], x);
 #pragma unroll
-          for (int k = 0; k < V; k += 2) {
-            const float2 y = __ffma2_rn(make_float2(x[k], x[k + 1]), make_float2(per_score, per_score), make_float2(c, c));
-            sum = __fadd2_rn(sum, make_float2(sm100::ex2_approx(y.x), sm100::ex2_approx(y.y)));
-          }
+        for (int k = 0; k < V; k += 2) {
+          const float2 d = __fadd2_rn(make_float2(x[k], x[k + 1]), make_float2(-base, -base));
+          const float2 y = __fmul2_rn(d, make_float2(per_score, per_score));
+          sum = __fadd2_rn(sum, make_float2(sm100::ex2_approx(y.x), sm100::ex2_approx(y.y)));
         }
       }
     }
-    if (where >= 0) {
-      float x[V];
-      unpack<T>(r.vector(where), x);
-#pragma unroll
-      for (int k = V - 1; k >= 0; --k)
-        if (fminf(x[k], FLT_MAX) == most) best = rank_key(most, r.head + where * V + k);
-    }
-    // c rounds -z_base per_score; what that leaves on every term is taken out
-    z = (sum.x + sum.y) * (z_base > -INFINITY ? sm100::ex2_approx(-__fmaf_rn(z_base, per_score, c)) : 1.f);
-    if (tid < r.ends) {
-      const float x = fminf(to_f32(r.x[r.end_index(tid)]), FLT_MAX);
-      if (to_f32(r.x[r.end_index(tid)]) > -INFINITY) {
-        const uint64_t key = rank_key(x, r.end_index(tid));
-        if (key > best) best = key;
-        if (z_base == -INFINITY) z_base = x;
-        z += sm100::ex2_approx((x - z_base) * per_score);
-      }
-    }
-    z_fine = z_base == -INFINITY ? z == 0.f : z > 0.f && z < 0x1p64f && fabsf(z_base * per_score) < 1e30f;
   }
+  if (where >= 0) {
+    float x[V];
+    unpack<T>(r.vector(where), x);
+#pragma unroll
+    for (int k = V - 1; k >= 0; --k)
+      if (fminf(x[k], FLT_MAX) == most) best = rank_key(most, r.head + where * V + k);
+  }
+  z = sum.x + sum.y;
+  if (tid < r.ends) {
+    const float x = fminf(r.end_score(tid), FLT_MAX);
+    if (r.end_score(tid) > -INFINITY) {
+      const uint64_t key = rank_key(x, r.end_index(tid));
+      if (key > best) best = key;
+      if (z_base == -INFINITY) z_base = x;
+      z += sm100::ex2_approx((x - z_base) * per_score);
+    }
+  }
+  z_fine = z_base == -INFINITY ? z == 0.f : z > 0.f && z < 0x1p64f;
   const uint64_t mine = best;
   best = team.max(best);
   if (!best || f.greedy) {
@@ -827,93 +837,91 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       __syncthreads();
       if (sh.bound) bounds[0] = key_value(sh.bound);
     }
-    {
-      for (int attempt = 0; attempt < 2 && bounds[attempt] > -INFINITY; ++attempt) {
-        const float from = bounds[attempt];
-        if (tid == 0) sh.counter = sh.hits = 0;
-        __syncthreads();
-        auto take = [&](int j, float x) {
-          if (x >= from) {
-            const int at = atomicAdd(&sh.counter, 1);
-            if (at < kSize) sh.list[at] = rank_key(x, j);
-          }
-        };
-        if (kMasked) {
-          each(r, tid, n, take);
-        } else {
-          if (tid < r.ends) take(r.end_index(tid), fminf(to_f32(r.x[r.end_index(tid)]), FLT_MAX));
-          auto take_vector = [&](int v, uint4 raw) {
-            float x[V];
-            unpack<T>(raw, x);
+    for (int attempt = 0; attempt < 2 && bounds[attempt] > -INFINITY; ++attempt) {
+      const float from = bounds[attempt];
+      if (tid == 0) sh.counter = sh.hits = 0;
+      __syncthreads();
+      auto take = [&](int j, float x) {
+        if (x >= from) {
+          const int at = atomicAdd(&sh.counter, 1);
+          if (at < kSize) sh.list[at] = rank_key(x, j);
+        }
+      };
+      if (tid < r.ends && r.end_score(tid) > -INFINITY) take(r.end_index(tid), fminf(r.end_score(tid), FLT_MAX));
+      auto take_vector = [&](int v, uint4 raw) {
+        float x[V];
+        unpack<T>(raw, x);
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-              if (x[k] == x[k]) take(r.head + v * V + k, fminf(x[k], FLT_MAX));
-          };
-          if (maxima) {  // each thread's own vectors' maxima; then their scores, all at once
+        for (int k = 0; k < V; ++k)
+          if (x[k] == x[k]) take(r.head + v * V + k, fminf(x[k], FLT_MAX));
+      };
+      if (maxima) {  // each thread's own vectors' maxima; then their scores, all at once
 #pragma unroll 8
-            for (int v = tid; v < r.vecs; v += n)
-              if (maxima[v] >= from) {
-                const int at = atomicAdd(&sh.hits, 1);
-                if (at < kSize) sh.hit[at] = v;
-              }
-            __syncthreads();
-            const int hits = sh.hits;
-            if (hits > kSize) {
-              __syncthreads();  // all have seen it
-              continue;
-            }
-            for (int h = tid; h < hits; h += n) take_vector(sh.hit[h], r.vector(sh.hit[h]));
-          } else {
-            constexpr int kAhead = 4;
-            for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
-              uint4 raw[kAhead];
-#pragma unroll
-              for (int i = 0; i < kAhead; ++i)
-                if (v0 + i * n < r.vecs) raw[i] = r.vector(v0 + i * n);
-#pragma unroll
-              for (int i = 0; i < kAhead; ++i)
-                if (v0 + i * n < r.vecs && max_vector<false, T>(-INFINITY, raw[i], 0) >= from) take_vector(v0 + i * n, raw[i]);
-            }
+        for (int v = tid; v < r.vecs; v += n)
+          if (maxima[v] >= from) {
+            const int at = atomicAdd(&sh.hits, 1);
+            if (at < kSize) sh.hit[at] = v;
           }
-        }
         __syncthreads();
-        const int m = sh.counter;
-        // Few by one warp, which has no barriers to wait for; in small blocks
-        // more too; in large ones all threads compare keys (256 rows of 131072
-        // with top_p 0.92: 35 us, against 43 with one warp for these; 4096 rows
-        // of 500 with top_p 0.9, two warps a row: 25 us, against 67 with both).
-        const bool few = m <= kFew, alone = few || (!by_count && n < 256 && m <= 2 * kRanked);
-        if (alone) {
-          if (tid < 32) {
-            bool done;
-            if (few) {
-              int j[kMine];
-              float x[kMine];
-#pragma unroll
-              for (int i = 0; i < kMine; ++i) {
-                const uint64_t key = tid + 32 * i < m ? sh.list[tid + 32 * i] : 0;
-                j[i] = key ? key_index(key) : -1;
-                x[i] = key_score(key);
-              }
-              done = draw_from_few(a, row, r, f, j, x, row_weight, *(FewShared*)(sh.list + kFew));
-            } else {
-              done = draw_by_weight(a, row, Team<true>{nullptr, tid, 32}, r, f, sh, m, from, top, row_weight);
-            }
-            if (tid == 0) sh.done = done;
-          }
-          __syncthreads();
-          if (sh.done) return;
+        const int hits = sh.hits;
+        if (hits > kSize) {
+          __syncthreads();  // all have seen it
+          continue;
         }
-        if (few) {
-        } else if (m <= kRanked && n >= 256) {
-          if (draw_by_rank(a, row, team, r, f, sh, m, top, row_weight)) return;
-        } else if (m <= kSize) {
-          if (!by_count && !alone && draw_by_weight(a, row, team, r, f, sh, m, from, top, row_weight)) return;
-          if (draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
+        for (int h = tid; h < hits; h += n) take_vector(sh.hit[h], r.vector(sh.hit[h]));
+      } else {
+        constexpr int kAhead = 4;
+        for (int v0 = tid; v0 < r.vecs; v0 += kAhead * n) {
+          uint4 raw[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+            if (v0 + i * n < r.vecs) raw[i] = r.vector(v0 + i * n);
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+            if (v0 + i * n < r.vecs && max_vector<false, T>(-INFINITY, raw[i], 0) >= from) take_vector(v0 + i * n, raw[i]);
         }
       }
+      __syncthreads();
+      const int m = sh.counter;
+      // Few by one warp, which has no barriers to wait for; in small blocks
+      // more too; in large ones all threads compare keys (256 rows of 131072
+      // with top_p 0.92: 35 us, against 43 with one warp for these; 4096 rows
+      // of 500 with top_p 0.9, two warps a row: 25 us, against 67 with both).
+      const bool few = m <= kFew, alone = few || (!by_count && n < 256 && m <= 2 * kRanked);
+      if (alone) {
+        if (tid < 32) {
+          bool done;
+          if (few) {
+            int j[kMine];
+            float x[kMine];
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              const uint64_t key = tid + 32 * i < m ? sh.list[tid + 32 * i] : 0;
+              j[i] = key ? key_index(key) : -1;
+              x[i] = key_score(key);
+            }
+            done = draw_from_few(a, row, r, f, j, x, row_weight, *(FewShared*)(sh.list + kFew));
+          } else {
+            done = draw_by_weight(a, row, Team<true>{nullptr, tid, 32}, r, f, sh, m, from, top, row_weight);
+          }
+          if (tid == 0) sh.done = done;
+        }
+        __syncthreads();
+        if (sh.done) return;
+      }
+      if (few) {
+      } else if (m <= kRanked && n >= 256) {
+        if (draw_by_rank(a, row, team, r, f, sh, m, top, row_weight)) return;
+      } else if (m <= kSize) {
+        if (!by_count && !alone && draw_by_weight(a, row, team, r, f, sh, m, from, top, row_weight)) return;
+        if (draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
+      }
     }
-    if (by_count) last = last_by_bins<false, kSize>(team, r, f, top, (double)f.top_k, -INFINITY, sh.list, &sh.counter);
+    if (by_count) {
+      // twice the depth of the least of the threads' best scores
+      const float depth = team.max(mine ? top - key_score(mine) : 0.f), span = 2.f * depth;
+      last = last_by_bins<false, kSize>(team, r, f, top, (double)f.top_k, -INFINITY, span, sh.list, &sh.counter);
+    }
     if (by_weight) {
       if (by_count) {
         uint64_t w = 0;
@@ -926,19 +934,11 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
       // than 1 - top_p of it together: the share is reached before them
       const float least = (float)((1.0 - f.top_p) * row_weight * 0x1p-44) / r.actions * 0.999f;
       const float from = least > 1e-30f ? top + (logf(fminf(least, 1.f)) - 0.001f) * f.temperature : -INFINITY;
-      const uint64_t cut = last_by_bins<true, kSize>(team, r, f, top, f.top_p * row_weight, from, sh.list, &sh.counter);
+      const uint64_t cut = last_by_bins<true, kSize>(team, r, f, top, f.top_p * row_weight, from, 31.f * f.temperature, sh.list, &sh.counter);
       if (cut > last) last = cut;
     }
   }
-  if (kMasked) {
-    Draw d;
-    each(r, tid, n, [&](int j, float x) {
-      if (rank_key(x, j) >= last) d.add(f, top, x, j, r.noise);
-    });
-    d.finish(a, row, team, r, f, top);
-  } else {
-    draw_from_all(a, row, team, r, f, top, last);
-  }
+  draw_from_all(a, row, team, r, f, top, last);
 }
 
 // A call of its own, so that rows that fit the list do not pay for its registers.
@@ -946,10 +946,9 @@ template <typename T, int kSize> __device__ __noinline__ void draw_masked_long(c
   draw_long<T, true>(a, row, sh, nullptr);
 }
 
-// Masked rows, in blocks of `row_warps` warps for every row: the mask gives the
-// visible actions' indices; up to kFew of them are left to one warp, which reads
-// their scores and noise at once.  Rows with more than fit a list are taken by
-// the whole block afterwards.
+// Masked rows, a warp each, four a block: the mask gives the visible actions'
+// indices; of up to kFew of them scores and noise are read at once.  Rows with
+// more than fit a list are taken by the whole block afterwards.
 template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sample_masked_kernel(const __grid_constant__ SampleArgs a) {
   constexpr int kRows = kMaskedThreads / 32, kIndices = 256;
   __shared__ union {
@@ -962,24 +961,21 @@ template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sampl
       };
     } part[kRows];
   } sh;
-  const int teams = blockDim.x / (32 * a.row_warps), lanes = 32 * a.row_warps;
-  const int team_id = threadIdx.x / lanes, tid = threadIdx.x % lanes;
-  const int64_t row = a.first_row + (int64_t)blockIdx.x * teams + team_id;
+  const int team_id = threadIdx.x / 32, tid = threadIdx.x % 32;
+  const int64_t row = a.first_row + (int64_t)blockIdx.x * kRows + team_id;
   const bool in = row < a.end_row;
-  const Row<T> r(a, in ? row : a.first_row);
+  const Row<T, false> r(a, in ? row : a.first_row);
   if (tid == 0) sh.part[team_id].count = 0;
-  if (lanes == 32) __syncwarp();
-  else __syncthreads();
+  __syncwarp();
   if (in)
-    each_visible<10>(r, tid, lanes, [&](int first, uint32_t bits) {
+    each_visible<10>(r, tid, 32, [&](int first, uint32_t bits) {
       int at = atomicAdd(&sh.part[team_id].count, __popc(bits));
       for (; bits; bits &= bits - 1, ++at)
         if (at < kIndices) sh.part[team_id].index[at] = first + __ffs(bits) - 1;
     });
-  if (lanes == 32) __syncwarp();
-  else __syncthreads();
+  __syncwarp();
   const int count = in ? sh.part[team_id].count : 0;
-  if (in && tid < 32 && count <= kIndices) {
+  if (in && count <= kIndices) {
     const Filters f(a.cfg, row);
     const int* index = sh.part[team_id].index;
     if (count <= kFew) {
@@ -1015,9 +1011,9 @@ template <typename T> __global__ void __launch_bounds__(kMaskedThreads, 8) sampl
   }
   const bool over = count > kIndices;
   if (!__syncthreads_or(over)) return;
-  for (int t = 0; t < teams; ++t)
+  for (int t = 0; t < kRows; ++t)
     if (__syncthreads_or(over && team_id == t)) {
-      draw_masked_long<T>(a, a.first_row + (int64_t)blockIdx.x * teams + t, sh.whole);
+      draw_masked_long<T>(a, a.first_row + (int64_t)blockIdx.x * kRows + t, sh.whole);
       __syncthreads();
     }
 }
@@ -1026,7 +1022,48 @@ template <typename T, int kSize, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_long_kernel(const __grid_constant__ SampleArgs a) {
   __shared__ Shared<kSize> sh;
   extern __shared__ float maxima[];
-  draw_long<T, false>(a, a.first_row + blockIdx.x, sh, a.rows.actions / Row<T>::V <= kMaximaVecs ? maxima : nullptr);
+  draw_long<T, false>(a, a.first_row + blockIdx.x, sh, a.rows.actions / (16 / (int)sizeof(T)) <= kMaximaVecs ? maxima : nullptr);
+}
+
+// Long masked rows, a block each: up to kRanked visible actions are listed, of
+// more the row's vectors are gone through as without a mask.
+template <typename T> __global__ void __launch_bounds__(kSampleThreads, 2) sample_long_masked_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ Shared<kList> sh;
+  extern __shared__ float maxima[];
+  const int64_t row = a.first_row + blockIdx.x;
+  const int tid = threadIdx.x, n = blockDim.x;
+  const Row<T, true> r(a, row);
+  if (tid == 0) sh.hits = sh.counter = 0;
+  __syncthreads();
+  each_visible<4>(r, tid, n, [&](int first, uint32_t bits) {
+    int at = atomicAdd(&sh.hits, __popc(bits));
+    for (; bits; bits &= bits - 1, ++at)
+      if (at < kRanked) sh.hit[at] = first + __ffs(bits) - 1;
+  });
+  __syncthreads();
+  const int visible = sh.hits;
+  if (visible > kRanked) {
+    __syncthreads();
+    draw_long<T, true>(a, row, sh, a.rows.actions / (16 / (int)sizeof(T)) <= kMaximaVecs ? maxima : nullptr);
+    return;
+  }
+  const Team<false> team{sh.slots, tid, n};
+  const Filters f(a.cfg, row);
+  uint64_t best = 0;
+  for (int i = tid; i < visible; i += n) {
+    const int j = sh.hit[i];
+    const float x = to_f32(r.x[j]);
+    if (!(x > -INFINITY)) continue;  // a NaN counts as -inf
+    const uint64_t key = rank_key(fminf(x, FLT_MAX), j);
+    sh.list[atomicAdd(&sh.counter, 1)] = key;
+    if (key > best) best = key;
+  }
+  best = team.max(best);
+  if (!best || f.greedy) {
+    if (tid == 0) answer(a, row, best ? key_index(best) : -1, 0.f);
+    return;
+  }
+  draw_by_rank(a, row, team, r, f, sh, sh.counter, key_score(best), -1.0);
 }
 
 template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cudaStream_t stream) {
@@ -1039,21 +1076,18 @@ template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cuda
     if (A <= kFew) {
       sample_warp_kernel<T><<<(unsigned)((n + 3) / 4), 128, 0, stream>>>(a);
     } else {
-      // a warp for up to 5120 mask bytes (ten loads a lane), else the whole block;
-      // without a mask eight scores or four vectors a thread
-      if (a.rows.mask) {
-        a.row_warps = A <= 5120 ? 1 : kMaskedThreads / 32;
-        const int teams = kMaskedThreads / 32 / a.row_warps;
-        sample_masked_kernel<T><<<(unsigned)((n + teams - 1) / teams), kMaskedThreads, 0, stream>>>(a);
+      // masked, a warp for up to 5120 actions (ten mask loads a lane)
+      if (a.rows.mask && A <= 5120) {
+        sample_masked_kernel<T><<<(unsigned)((n + 3) / 4), kMaskedThreads, 0, stream>>>(a);
       } else {
         // 32 scores a thread, so that there are many best scores to choose from
         const int threads = min(kSampleThreads, max(32, (A / 32 + 31) / 32 * 32));
-        const int vecs = A / Row<T>::V;
+        const int vecs = A / (16 / (int)sizeof(T));
         const size_t smem = vecs <= kMaximaVecs ? (size_t)vecs * 4 : 0;
         if (threads <= 64) {
           sample_long_kernel<T, 512, 64><<<(unsigned)n, threads, smem, stream>>>(a);
         } else {
-          auto kernel = sample_long_kernel<T, kList, kSampleThreads>;
+          auto kernel = a.rows.mask ? sample_long_masked_kernel<T> : sample_long_kernel<T, kList, kSampleThreads>;
           if (smem > 24 * 1024)
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaximaVecs * 4);
           if (e != cudaSuccess) break;
@@ -1085,7 +1119,7 @@ extern "C" gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sampl
   if (noise_stride < 0) return bad(who, "negative stride");
   if (rows->rows == 0) return GZ_OK;
   if (!d_action) return bad(who, "null actions");
-  const SampleArgs a{row_args(rows), *cfg, d_noise, noise_stride, d_action, d_logp, 0, 0, 1};
+  const SampleArgs a{row_args(rows), *cfg, d_noise, noise_stride, d_action, d_logp, 0, 0};
   const cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (rows->dtype == GZ_F32) e = launch_sample<float>(a, rows->rows, s);
