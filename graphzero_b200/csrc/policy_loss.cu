@@ -278,17 +278,17 @@ __global__ void __launch_bounds__(128) loss_warp_kernel(LossArgs a) {
 
 // Longer rows: a block each, or a slice of a row per block of a cluster, in
 // two ways.
-//  - Dense: the slice's scores are copied to shared memory (asynchronously, all
-//    at once, so that few registers keep many bytes in flight) and passed over
-//    twice there, for the sums and for the gradient.  Targets are read in both,
-//    the second time from the caches; so are scores under a mask.  Scores, mask
-//    and targets are read and the gradient is written once: bound by memory,
-//    next by the two exponentials an action.
+//  - Dense: scores (from shared memory, where a copy without registers has put
+//    them), mask and targets are passed over twice, for the sums and for the
+//    gradient; what is not in shared memory comes from the caches the second
+//    time.  Scores, mask and targets are read and the gradient is written once:
+//    bound by memory, next by the two exponentials an action.
 //  - Listed: under a mask that leaves at most kListed actions of the slice
 //    visible (legal moves: some 30 of 4672) only these are read at all.  The
 //    mask gives their list in an order fixed by position, scores and targets
 //    are gathered, the gradient is zeros with the listed ones stored over
-//    them: the mask's byte and the gradient's bytes are what is left to move.
+//    them: the mask's byte and the gradient's bytes are what is left to move,
+//    209 MB of 497 on 8192 rows of 4672 in 46 us, 4.6 TB/s.
 // A cluster's blocks exchange maximum and sums through distributed shared
 // memory, once.
 constexpr int kListed = 256;
@@ -679,7 +679,7 @@ cudaError_t launch_loss(LossArgs a, int64_t rows, cudaStream_t stream) {
       e = cudaGetLastError();
       continue;
     }
-    // the slice: small enough that four blocks fit an SM's shared memory, and
+    // the slice: small enough that two blocks fit an SM's shared memory, and
     // with few rows smaller still, until the blocks fill the device
     int cluster = 1;
     while (cluster < 16 && (vecs + cluster - 1) / cluster > kSliceVecs) cluster *= 2;

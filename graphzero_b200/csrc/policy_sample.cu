@@ -2,25 +2,30 @@
 //
 // A row's order is that of its rank keys: the score's bits in an order-
 // preserving form, then the index, so that no two are alike, and the kept
-// actions of top_k and top_p are those from some rank key on.  Few candidates
-// are put into a list in shared memory and sorted; which way a row gets there:
-//  - Masked rows list their visible actions (16 mask bytes at a time; scores are
-//    read only where something is visible), and rows of at most kList actions
-//    list all of them.
-//  - Longer rows are read once for their best score and, where top_p needs it,
-//    their sum of exponentials.  The K-th largest of the threads' best scores
-//    has at least K actions at or above it: those are listed in a second pass,
-//    from the caches.  top_k takes K = top_k.  For top_p, K is half of the
-//    threads, and the list is enough if it reaches the share wanted.
-//  - Where it is not (flat rows, a large top_k), a histogram over the scores
-//    finds the bin that the last kept action lies in, and only that bin is
-//    listed and sorted; if a bin overflows the list (equal scores), the last
-//    rank key is found by bisection.
-// The draw is an argmax over the kept actions; noise is read for these alone.
+// actions of top_k and top_p are those from some rank key on.  Reading a row is
+// bound by memory, choosing from it by the latency of its steps; so a row is
+// read once, the few actions that can be kept go to a list in shared memory,
+// and the rest is done there, by one warp where the list is short:
+//  - Masked rows of up to 5120 actions (legal moves): a warp lists the visible
+//    ones, sixteen mask bytes at a time, and reads scores and noise of these
+//    alone.  4096 rows of 4672 with top_p and min_p: 13 us, 4.4 TB/s of scores
+//    and mask.
+//  - Other rows: a block reads the row once for its best score, its vectors'
+//    maxima and, where top_p needs it, its sum of exponentials.  A bound below
+//    which (nearly always) nothing is kept gives the list (draw_long).  256 rows
+//    of 131072 bf16 scores with top_p 0.92: 33 us, of which 17 read the rows
+//    (10 at the copy rate); the rest is steps of one after the other.
+//  - Where the list is too long or not enough (a wide share of a flat row, a
+//    large top_k), a histogram over the scores finds the bin that the last kept
+//    action lies in, and only that bin is listed and sorted; if it overflows the
+//    list (equal scores), the last rank key is found by bisection.
+// The draw is an argmax over the kept actions; noise is read for these alone,
+// or, where nearly all are kept, a vector at a time.
 //
-// Weights exp(d) of listed actions are summed as integers in units of 2^-44, so
-// that neither the list's order nor the atomics' matters; sums over whole rows
-// are 32-bit floats in an order given by the row's length and alignment.
+// Weights exp(d) of listed actions are summed as whole numbers of 2^-44, so
+// that neither the list's order nor that of the atomics matters; sums over
+// whole rows are 32-bit floats in an order given by the row's length and
+// alignment.
 #include "gz_policy.h"
 
 namespace gz {
@@ -37,8 +42,8 @@ struct SampleArgs {
   int64_t first_row, end_row;  // of this launch
 };
 
-constexpr int kList = 2048;         // keys a block's list holds
-constexpr int kMaskedList = 1024, kMaskedThreads = 128;  // the same for masked rows, and their blocks
+constexpr int kList = 2048;          // keys a block's list holds
+constexpr int kMaskedList = 1024, kMaskedThreads = 128;  // the same for blocks of four masked rows, and their threads
 constexpr int kSampleThreads = 512;  // most threads of a block
 constexpr int kReachBit = 16;       // lowest bit of a score that the search for a list's bound looks at
 constexpr int kMaximaVecs = 24576;  // vectors of a row whose maxima are kept (96 KB: two blocks fit an SM)
@@ -491,15 +496,16 @@ template <int kSize> struct Shared {
   uint32_t bound, sums[3];
 };
 
-// Draws from an unmasked row's actions from the rank key `last` on (0: all): the
-// scores from the caches once more, and the noise.  The kept weight is summed
-// in 32 bits (under a mask in whole numbers).  Noisy scores are compared as they are defined, but with a
-// temperature the division is done only for vectors whose upper bound, from a
-// product with its reciprocal, could still win.
+// Draws from a row's actions from the rank key `last` on (0: all): the scores
+// from the caches once more, and the noise.  The kept weight is summed in 32
+// bits (under a mask in whole numbers).  Noisy scores are compared as they are
+// defined, but with a temperature the division is done only for vectors whose
+// upper bound, from a product with its reciprocal, could still win.  256
+// unfiltered rows of 131072: 63 us, 1.6 TB/s, bound by instructions.
 template <typename T, bool kMask>
 __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T, kMask>& r, const Filters& f, float top,
                               uint64_t last) {
-  constexpr int V = (16 / (int)sizeof(T));
+  constexpr int V = 16 / (int)sizeof(T);
   const int tid = team.tid, n = team.n;
   const float* noise = r.noise ? r.noise + r.head : nullptr;
   const bool aligned = ((uintptr_t)noise & 15) == 0;
@@ -590,7 +596,6 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
   }
 }
 
-// A row whose visible actions do not all fit the list.
 // Draws from a list of m actions, at most kRanked, in any order, with the block:
 // a key's rank and the weight before it come from comparing it with all others.
 // row_weight and the answer as in draw_from_list.
@@ -663,7 +668,7 @@ __device__ bool draw_by_weight(const SampleArgs& a, int64_t row, const Team<kWar
     __syncthreads();
     return *sum;
   };
-  // (the sum cannot pass 2^32: it is at most the row's weight, below 2^31 / top_p)
+  // (a sum that passes 2^32 only looks too small: the score is raised less)
   const uint32_t low = order_key(from), high = order_key(top);
   if (above(low) < goal22) return false;
   const int first = 31 - __clz(low ^ high | 1);
@@ -699,11 +704,11 @@ __device__ bool draw_by_weight(const SampleArgs& a, int64_t row, const Team<kWar
   return true;
 }
 
-// maxima: a float for every vector of the row, or null.  kMask: it is read
-// through its mask.
+// A row with a block.  maxima: a float for every vector of the row, or null.
+// kMask: it is read through its mask.
 template <typename T, bool kMask, int kSize>
 __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shared<kSize>& sh, float* maxima) {
-  constexpr int V = (16 / (int)sizeof(T));
+  constexpr int V = 16 / (int)sizeof(T);
   const int tid = threadIdx.x, n = blockDim.x;
   const Team<false> team{sh.slots, tid, n};
   const Row<T, kMask> r(a, row);
