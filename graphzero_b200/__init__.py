@@ -739,17 +739,17 @@ class _On:
 
 
 def _on(f):
-    """Runs f(tensor, ..., stream=...) with the tensor's device and the stream current."""
+    """Runs f(logits, ..., stream=...) with the logits' device and the stream current."""
 
     @functools.wraps(f)
-    def run(x, *args, stream=None, **kw):
+    def run(logits, *args, stream=None, **kw):
         torch = _torch or _need_torch()
-        if stream is None and (not x.is_cuda or x.device.index == torch._C._cuda_getDevice()):
-            return f(x, *args, **kw)
-        if not x.is_cuda:
-            raise ValueError("CUDA tensors are needed")
-        with _On(x.device, stream):
-            return f(x, *args, **kw)
+        if not logits.is_cuda:
+            raise ValueError("logits must be a CUDA tensor")
+        if stream is None and logits.device.index == torch._C._cuda_getDevice():
+            return f(logits, *args, **kw)
+        with _On(logits.device, stream):
+            return f(logits, *args, **kw)
 
     return run
 

@@ -691,7 +691,8 @@ cudaError_t launch_loss(LossArgs a, int64_t rows, cudaStream_t stream) {
     const size_t smem = masked ? 0 : (size_t)per * 16;
     a.cluster = cluster;
     auto kernel = masked ? loss_masked_kernel<T, kDense> : loss_kernel<T, kDense>;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (48 KB go without asking, the kernel's own few included)
+    if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess && cluster == 16)
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) break;

@@ -1093,7 +1093,8 @@ template <typename T> cudaError_t launch_sample(SampleArgs a, int64_t rows, cuda
           sample_long_kernel<T, 512, 64><<<(unsigned)n, threads, smem, stream>>>(a);
         } else {
           auto kernel = a.rows.mask ? sample_long_masked_kernel<T> : sample_long_kernel<T, kList, kSampleThreads>;
-          if (smem > 24 * 1024)
+          // (48 KB go without asking, some 25 KB of the kernel's own included)
+          if (smem > 16 * 1024)
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaximaVecs * 4);
           if (e != cudaSuccess) break;
           kernel<<<(unsigned)n, threads, smem, stream>>>(a);

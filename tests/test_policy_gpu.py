@@ -218,6 +218,38 @@ def test_sample_frequencies(cuda):
         assert (logp.double().cpu() - p.log()[action.long().cpu()]).abs().max() < 1e-5
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_step_of_shared_memory(cuda, dtype):
+    """Rows whose shared memory lies on either side of what a launch gets without asking."""
+    per = 4 // dtype.itemsize * 4  # actions of a 16-byte vector
+    for vecs in (2500, 2900, 3000, 3072, 3500, 5900, 5980, 6050, 6144, 6300, 12200, 24576, 24577):
+        a = vecs * per
+        if a > gz.POLICY_MAX_ACTIONS:
+            continue
+        x = rows_of(2, a, vecs, dtype)
+        check_sample(x, ref.gumbel((2, a), 1), top_k=3)
+        n = 150  # as many rows as multiprocessors: none is split for want of rows
+        y = x[:1].cuda().expand(n, a)
+        loss, grad = gz.policy_loss(y, label=torch.zeros(n, dtype=torch.int32, device="cuda"))
+        want, wgrad, terms = ref.loss(x[:1].float().numpy(), None, label=np.zeros(1, np.int64))
+        assert (np.abs(loss.cpu().numpy() - want[0]) <= (a / 32 + 64) * U * terms[0]).all()
+        assert torch.equal(grad[0], grad[-1])
+
+
+def test_keywords_and_streams_by_number(cuda):
+    x, noise = rows_of(3, 300, 1).cuda(), ref.gumbel((3, 300), 2).cuda()
+    want = gz.policy_sample(x, noise, top_p=0.5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (side, side.cuda_stream):
+        got = gz.policy_sample(logits=x, noise=noise, top_p=0.5, stream=stream)
+        side.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        loss, _ = gz.policy_loss(logits=x.t().contiguous().t(), label=want[0], stream=stream)
+        side.synchronize()
+        assert torch.equal(loss, gz.policy_loss(x, label=want[0])[0])
+
+
 def test_offsets_beyond_32_bits(cuda):
     """Rows further apart than 2^31 elements."""
     a, stride = 1000, 2**31 + 24
