@@ -921,6 +921,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
         if (!by_count && !alone && draw_by_weight(a, row, team, r, f, sh, m, from, top, row_weight)) return;
         if (draw_from_list(a, row, team, r, f, sh.list, m, m, top, row_weight)) return;
       }
+      __syncthreads();  // all have read the count, and the list
     }
     if (by_count) {
       // twice the depth of the least of the threads' best scores
