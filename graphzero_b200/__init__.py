@@ -13,7 +13,6 @@ broadcast_weights) and its factory create_neural_net(type, game)
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import os
 import struct
 from pathlib import Path
@@ -738,27 +737,18 @@ class _On:
         self._device.__exit__(*exc)
 
 
-def _on(f):
-    """Runs f(logits, ..., stream=...) with the logits' device and the stream current."""
-
-    @functools.wraps(f)
-    def run(logits, *args, stream=None, **kw):
-        torch = _torch or _need_torch()
-        if not logits.is_cuda:
-            raise ValueError("logits must be a CUDA tensor")
-        if stream is None and logits.device.index == torch._C._cuda_getDevice():
-            return f(logits, *args, **kw)
-        with _On(logits.device, stream):
-            return f(logits, *args, **kw)
-
-    return run
+def _elsewhere(logits, stream):
+    """Whether a call needs another device or stream than the current ones (an _On)."""
+    if not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor")
+    return stream is not None or logits.device.index != _torch._C._cuda_getDevice()
 
 
 def _policy_rows(logits, mask):
     """What gz_policy_rows points to, and its packed form."""
     dtype = _float_dtypes.get(logits.dtype)
-    if dtype is None or logits.dim() != 2 or not logits.is_cuda:
-        raise ValueError("logits must be a [rows][actions] CUDA tensor of float32, float16 or bfloat16")
+    if dtype is None or logits.dim() != 2:
+        raise ValueError("logits must be a [rows][actions] tensor of float32, float16 or bfloat16")
     n, a = logits.shape
     if a > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
@@ -785,8 +775,7 @@ def _action_values(x, name, logits):
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-@_on
-def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=None):
     """One action per row of `logits` (torch, [rows][actions], float32, float16
     or bfloat16), drawn with `noise` (float32 standard Gumbel numbers of the
     same shape, e.g. -torch.empty(...).exponential_().log(); None picks the
@@ -794,8 +783,13 @@ def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p
     temperature, top_k, top_p and min_p keep.  Each setting is a number or a
     [rows] tensor (float32; top_k int32).  Returns (action int32 [rows], -1
     where nothing is visible; logp float32 [rows], the action's
-    log-probability among the kept ones).  `stream` (keyword): a stream to run
-    on instead of the current one.  See gz_policy_sample."""
+    log-probability among the kept ones).  `stream`: a stream to run on instead
+    of the current one.  See gz_policy_sample."""
+    if _torch is None:
+        _need_torch()
+    if _elsewhere(logits, stream):
+        with _On(logits.device, stream):
+            return policy_sample(logits, noise, mask, temperature, top_k, top_p, min_p)
     logits, mask, rows = _policy_rows(logits, mask)
     n, dev, tensor = logits.shape[0], logits.device, _torch.Tensor
     d_temperature = d_top_k = d_top_p = d_min_p = 0
@@ -823,16 +817,20 @@ def policy_sample(logits, noise=None, mask=None, temperature=1.0, top_k=0, top_p
     return action, logp
 
 
-@_on
-def policy_loss(logits, target=None, label=None, mask=None, weight=None, grad_scale=1.0, need_grad=True):
+def policy_loss(logits, target=None, label=None, mask=None, weight=None, grad_scale=1.0, need_grad=True, stream=None):
     """Cross-entropy of softmax(logits) over the actions that `mask` leaves
     visible, and its gradient, in one pass: (loss float32 [rows], grad of the
     logits' shape and type, or None without need_grad).  The targets are
     `target` (float32 [rows][actions] amounts) or `label` (int32 [rows]);
     `weight` (float32 [rows]) multiplies a row, `grad_scale` the gradient
     alone (1 / rows for the mean loss).  Continue a torch backward pass with
-    logits.backward(grad).  `stream` (keyword): a stream to run on instead of
-    the current one.  See gz_policy_loss."""
+    logits.backward(grad).  `stream`: a stream to run on instead of the current
+    one.  See gz_policy_loss."""
+    if _torch is None:
+        _need_torch()
+    if _elsewhere(logits, stream):
+        with _On(logits.device, stream):
+            return policy_loss(logits, target, label, mask, weight, grad_scale, need_grad)
     logits, mask, rows = _policy_rows(logits, mask)
     (n, a), dev = logits.shape, logits.device
     if (target is None) == (label is None):
