@@ -414,8 +414,10 @@ __device__ __forceinline__ bool in_range(float z) { return z > 0.f && z < 0x1p64
 
 // The dense way under a mask: scores, mask and targets are read from memory for
 // the sums and again, from the caches, for the gradient.  The sums' first
-// reference is the largest of a sample, each thread's first vector.  A call of
-// its own, so that the listed way does not pay for its registers.
+// reference is the largest of a sample, each thread's first vector; where the
+// sample has nothing above -inf (the row may begin with hidden actions) the
+// maximum is looked for before any sum counts.  A call of its own, so that the
+// listed way does not pay for its registers.
 template <typename T, bool kDense>
 __device__ __noinline__ void masked_dense_slice(const LossArgs& a, LossShared& sh) {
   const int tid = threadIdx.x, n = blockDim.x;
@@ -443,7 +445,7 @@ __device__ __noinline__ void masked_dense_slice(const LossArgs& a, LossShared& s
     p.z = z.x + z.y;
     p = block_sum<kDense>(p, sh);
     p.z *= scale.fix;
-    if (!sample || in_range(p.z)) break;
+    if (!sample || (m > -INFINITY && in_range(p.z))) break;
     p.m = fmaxf(ex, -INFINITY);
     for (int v = tid; v < r.vecs; v += n) p.m = max_vector<true, T>(p.m, __ldg(from + v), r.seen(v));
     __syncthreads();  // the sums have been read
