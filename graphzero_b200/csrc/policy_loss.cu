@@ -35,12 +35,15 @@ __device__ __forceinline__ float exp_of(float d) { return sm100::ex2_approx(d * 
 
 // exp(x - ref) as one multiply-add and a power of two, 2^(a x + c): c rounds
 // -a ref, and the factor 2^(a ref + c) that this leaves on every term is taken
-// out of the sums by `fix`.  At |ref| from 1e30 on, where a ref could overflow,
-// the floats nearest to ref are so far from it that a = 1 gives the same 1 and 0.
+// out of the sums by `fix`.  Its exponent is up to half a unit in the last place
+// of 1.44 |ref|, so below |ref| = 2^30 at most 64, and both powers stay far
+// within range.  From 2^30 on the next float below ref is 64 or more away: all
+// that differs from ref adds nothing to a sum that ref's 1 is in, at a = 1
+// (2^-64) as at a = log2 e (e^-64), and a = 1 needs no rounding.
 struct Scale {
   float a, c, fix;
   __device__ explicit Scale(float ref) {
-    a = fabsf(ref) < 1e30f ? 1.44269504f : 1.f;
+    a = fabsf(ref) < 0x1p30f ? 1.44269504f : 1.f;
     c = -__fmul_rn(ref, a);
     fix = sm100::ex2_approx(-__fmaf_rn(ref, a, c));
   }

@@ -1,9 +1,12 @@
 """The policy loss and sampling at the edges of their inputs, against the plain
 restatements in 64 bits (tests/policy_ref.py)."""
+import numpy as np
 import pytest
 import torch
 
-from test_policy_gpu import DTYPES, check_loss, rows_of
+import graphzero_b200 as gz
+import policy_ref as ref
+from test_policy_gpu import DTYPES, U, check_loss, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +50,56 @@ def test_loss_rows_that_begin_with_hidden_actions(cuda, n, a, slice_size, prefix
     assert (loss > 0).all() and (grad != 0).any(1).all()
     loss, grad = check_loss(x, mask, label=label)
     assert (loss > 0).all() and (grad[:, a - 1] < 0).all()
+
+
+LARGE = [2.0**29, 1e9, 2.0**30, 2.0**31 - 128, 2.0**31, 5e9, 1e10, 1e11, 1e15, 1e20, 1e29, 1e30, 3e38]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,a,share", [
+    (3 * 2 * len(LARGE), 300, None), (3 * 2 * len(LARGE), 300, 0.5),  # a warp a row
+    (3 * 2 * len(LARGE), 4672, 0.02),                                 # listed
+    (6 * 2 * len(LARGE), 9000, 0.5), (3 * 2 * len(LARGE), 60000, 0.5),   # through a mask: a block a row, slices
+    (6 * 2 * len(LARGE), 9000, None), (3 * 2 * len(LARGE), 60000, None),  # without
+])
+def test_loss_of_scores_of_any_magnitude(cuda, n, a, share, dtype):
+    """Rows around +-2^29 to +-3e38: all alike (a finished game in a batch that
+    hides moves by a large negative score), with a third of the scores lower
+    still, and ordinary scores beside a third at the large negative value.
+
+    Tolerance: that of check_loss with the depth of scores that count (24; e^-24
+    of the sum is below u).  From 2^30 on neighbouring floats lie 64 or more
+    apart, so all but the best have shares below e^-64 and may come out as
+    anything up to 2^-64."""
+    base = torch.tensor([s * v for v in LARGE for s in (1, -1)])
+    kind = torch.arange(n) // len(base) % 3
+    base = base.repeat(-(-n // len(base)))[:n, None].to(dtype).float()
+    low = torch.arange(a)[None, :] % 3 == 1
+    x = base.repeat(1, a)
+    x = torch.where((kind == 1)[:, None] & low, (base - 0.1 * base.abs()).to(dtype).float(), x)
+    ordinary = rows_of(n, a, a).clamp(-6, 6)
+    x = torch.where((kind == 2)[:, None], torch.where(low, -base.abs(), ordinary), x).to(dtype)
+    g = torch.Generator().manual_seed(1)
+    mask = None
+    if share is not None:
+        mask = (torch.rand(n, a, generator=g) < share).to(torch.uint8)
+        mask[:, 0] = mask[:, 1] = 1
+    target = torch.where(low, torch.zeros(()), torch.rand(n, a, generator=g)) / a
+    label = torch.zeros(n, dtype=torch.int32)
+    xs = x.float().numpy()
+    few = (a / 32 + 64) * U
+    half, least = {torch.float32: (U, 2.0**-149), torch.bfloat16: (2.0**-8, 2.0**-134)}[dtype]
+    for t, l in ((target, None), (None, label)):
+        up = lambda v: None if v is None else v.cuda()  # noqa: E731
+        arr = lambda v: None if v is None else v.numpy()  # noqa: E731
+        loss, grad = gz.policy_loss(x.cuda(), target=up(t), label=up(l), mask=up(mask))
+        want, wgrad, terms = ref.loss(xs, arr(mask), arr(t), arr(l))
+        assert (np.abs(loss.cpu().numpy() - want) <= few * terms + 1e-38).all()
+        amount = np.zeros_like(wgrad)
+        if t is None:
+            amount[:, 0] = 1.0
+        else:
+            amount = np.where(np.ones_like(xs, bool) if mask is None else mask.numpy() != 0, t.numpy(), 0.0)
+        p = np.abs(wgrad + amount) + amount
+        bound = 25 * few * p + half * np.abs(wgrad) + least + 2.0**-64
+        assert (np.abs(grad.float().cpu().numpy() - wgrad) <= bound).all()
