@@ -891,12 +891,12 @@ class AdamW:
         for p in self.params:
             self.offsets.append(total)
             total += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
-        self.m, self.v = torch.zeros(total, device=self.device), torch.zeros(total, device=self.device)
+        f32 = dict(dtype=torch.float32, device=self.device)  # named: the default type is the program's
+        self.m, self.v = torch.zeros(total, **f32), torch.zeros(total, **f32)
         self.m_scale = self.v_scale = None
         if state_bits == 8:
             self.m, self.v = self.m.to(torch.float8_e4m3fn), self.v.to(torch.float8_e4m3fn)
-            self.m_scale = torch.ones(total // ADAMW_BLOCK, device=self.device)
-            self.v_scale = torch.ones(total // ADAMW_BLOCK, device=self.device)
+            self.m_scale, self.v_scale = torch.ones(total // ADAMW_BLOCK, **f32), torch.ones(total // ADAMW_BLOCK, **f32)
         table = (AdamWTensor * count)()
         size = self.m.element_size()
         for t, p, c, at, decay, scale in zip(table, self.params, self.copies, self.offsets, decays, scales):
@@ -948,7 +948,7 @@ class AdamW:
             return self._step(grad_scale)
 
     def _step(self, grad_scale):
-        norm = _torch.empty((), device=self.device) if self.max_norm > 0 else None
+        norm = _torch.empty((), dtype=_torch.float32, device=self.device) if self.max_norm > 0 else None
         c = self._cfg
         c.lr, (c.beta1, c.beta2), c.eps = self.lr, self.betas, self.eps
         c.max_norm, c.grad_scale, c.step, c.seed = self.max_norm, grad_scale, self.steps + 1, self.seed
