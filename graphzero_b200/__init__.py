@@ -863,16 +863,19 @@ class AdamW:
     ADAMW_BLOCK and starting at offsets[k]: m and v (32 bits), or m and the
     root of v as float8_e4m3fn with m_scale and v_scale per block (8 bits).
     Together with `steps`, the number of steps taken, they are all there is to
-    save.  `lr` and `max_norm` may be changed between steps."""
+    save; restore them in place (opt.m.copy_(saved), opt.steps = n).  The
+    kernels hold the addresses of weights, copies and states: a step raises if
+    one of them has moved to other memory (p.data = ..., a module moved between
+    devices).  `lr` and `max_norm` may be changed between steps."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, copies=None,
                  lr_scale=1.0, max_norm=0.0, seed=0):
         torch = _need_torch()
         self._plan = _vp()
-        self.params = list(params)
+        self._params = tuple(params)
         count = len(self.params)
         each = lambda x: list(x) if isinstance(x, (list, tuple)) else [x] * count  # noqa: E731
-        self.copies, decays, scales = each(copies), each(weight_decay), each(lr_scale)
+        self._copies, decays, scales = tuple(each(copies)), each(weight_decay), each(lr_scale)
         if not self.params:
             raise ValueError("no tensors")
         if any(len(x) != count for x in (self.copies, decays, scales)):
@@ -892,11 +895,11 @@ class AdamW:
             self.offsets.append(total)
             total += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
         f32 = dict(dtype=torch.float32, device=self.device)  # named: the default type is the program's
-        self.m, self.v = torch.zeros(total, **f32), torch.zeros(total, **f32)
-        self.m_scale = self.v_scale = None
+        self._m, self._v = torch.zeros(total, **f32), torch.zeros(total, **f32)
+        self._m_scale = self._v_scale = None
         if state_bits == 8:
-            self.m, self.v = self.m.to(torch.float8_e4m3fn), self.v.to(torch.float8_e4m3fn)
-            self.m_scale, self.v_scale = torch.ones(total // ADAMW_BLOCK, **f32), torch.ones(total // ADAMW_BLOCK, **f32)
+            self._m, self._v = self.m.to(torch.float8_e4m3fn), self.v.to(torch.float8_e4m3fn)
+            self._m_scale, self._v_scale = torch.ones(total // ADAMW_BLOCK, **f32), torch.ones(total // ADAMW_BLOCK, **f32)
         table = (AdamWTensor * count)()
         size = self.m.element_size()
         for t, p, c, at, decay, scale in zip(table, self.params, self.copies, self.offsets, decays, scales):
@@ -908,8 +911,19 @@ class AdamW:
             if c is not None:
                 t.copy, t.copy_dtype = c.data_ptr(), _float_dtypes[c.dtype]
         _check(_lib.gz_adamw_create(table, count, state_bits, self.device.index, C.byref(self._plan)))
+        held = (*self.params, *self.copies, self.m, self.v, self.m_scale, self.v_scale)
+        self._held = [t for t in held if t is not None]
+        self._addresses = [t.data_ptr() for t in self._held]
         self._shapes = [p.shape for p in self.params]
         self._grads, self._kinds, self._cfg = (_vp * count)(), (C.c_int32 * count)(), AdamWConfig()
+
+    # what the plan points to: to be written in place, not replaced
+    params = property(lambda self: self._params)
+    copies = property(lambda self: self._copies)
+    m = property(lambda self: self._m)
+    v = property(lambda self: self._v)
+    m_scale = property(lambda self: self._m_scale)
+    v_scale = property(lambda self: self._v_scale)
 
     def close(self) -> None:
         if self._plan:
@@ -942,6 +956,9 @@ class AdamW:
                 raise ValueError("gradients must be contiguous tensors of their weights' shapes in float32, float16 "
                                  "or bfloat16")
             pointers[k], kinds[k] = g.data_ptr(), kind
+        if list(map(_torch.Tensor.data_ptr, self._held)) != self._addresses:
+            raise ValueError("a weight, copy or state has moved to other memory since this AdamW was made: write them in "
+                             "place, or make a new AdamW and copy the states into it")
         if stream is None and device.index == _torch._C._cuda_getDevice():
             return self._step(grad_scale)
         with _On(device, stream):

@@ -27,3 +27,62 @@ def test_states_do_not_follow_the_default_type(cuda, bits, default):
         torch.set_default_dtype(torch.float32)
     assert norm.dtype == torch.float32 and torch.equal(norm, want.step(gs))
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(want.m.float(), got.m.float())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_tensors_that_have_moved_are_refused(cuda, bits):
+    """A plan holds its tensors' addresses: a step after one got other memory
+    raises and changes nothing (the old memory is kept here throughout)."""
+    shapes = [(300, 3), (17,)]
+    gs = gradients(shapes, 1)
+
+    def moved(take, put):
+        params = make(shapes)
+        copies = [p.to(torch.bfloat16) for p in params]
+        opt = gz.AdamW(params, state_bits=bits, copies=copies)
+        opt.step(gs)
+        t = take(opt, params, copies)
+        old = t.data
+        kept = old.float().clone()
+        put(t)
+        with pytest.raises(ValueError, match="moved"):
+            opt.step(gs)
+        assert opt.steps == 1 and torch.equal(old.float(), kept)
+        t.data = old  # back again
+        opt.step(gs)
+        assert opt.steps == 2
+
+    other = lambda t: setattr(t, "data", t.data.clone())  # noqa: E731
+    moved(lambda o, p, c: p[1], other)
+    moved(lambda o, p, c: p[0], other)
+    moved(lambda o, p, c: c[1], other)
+    moved(lambda o, p, c: o.m, other)
+    moved(lambda o, p, c: o.v, other)
+    moved(lambda o, p, c: p[1], lambda t: t.set_(t.clone()))
+    if bits == 8:
+        moved(lambda o, p, c: o.m_scale, other)
+        moved(lambda o, p, c: o.v_scale, other)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_are_restored_in_place(cuda, bits):
+    shapes = [(300, 3), (17,)]
+    a, gs = make(shapes), gradients(shapes, 1)
+    opt = gz.AdamW(a, state_bits=bits)
+    opt.step(gs)
+    saved = {k: getattr(opt, k).clone() for k in ("m", "v", "m_scale", "v_scale") if getattr(opt, k) is not None}
+    weights = [p.clone() for p in a]
+    opt.step(gs)
+    for k, t in saved.items():
+        with pytest.raises(AttributeError):
+            setattr(opt, k, t)
+    again = gz.AdamW(weights, state_bits=bits)
+    for k, t in saved.items():
+        getattr(again, k).copy_(t)
+    again.steps = 1
+    again.step(gs)
+    assert all(torch.equal(p, q) for p, q in zip(a, weights)) and torch.equal(opt.m.float(), again.m.float())
+    with pytest.raises(AttributeError):
+        opt.params = weights
+    with pytest.raises(TypeError):
+        opt.params[0] = weights[0]
