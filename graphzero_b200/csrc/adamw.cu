@@ -59,7 +59,7 @@ struct StepArgs {
   uint32_t blocks;         // blocks per chunk
   double lr, lr_corrected;  // lr, lr / (1 - beta1^t)
   float beta1, one_beta1, beta2, one_beta2, eps, correct2;  // correct2 = 1 / sqrt(1 - beta2^t)
-  float grad_scale, max_norm;
+  float grad_scale, max_norm;  // max_norm 0: no clipping
   uint32_t key;            // of the rounding
   double* partial;         // sums of squares, one per chunk of the plan
   unsigned* arrived;
@@ -273,7 +273,10 @@ struct Rates {
     decay = (float)(1.0 - a.lr * t.lr_scale * t.weight_decay);
     step = (float)(a.lr_corrected * t.lr_scale);
     scale = a.grad_scale;
-    if (a.max_norm > 0.f) scale = __fmul_rn(scale, fminf(__fdiv_rn(a.max_norm, __fadd_rn(*a.norm, 1e-6f)), 1.f));
+    if (a.max_norm > 0.f) {
+      const float clip = __fdiv_rn(a.max_norm, __fadd_rn(*a.norm, 1e-6f));
+      scale = __fmul_rn(scale, clip > 1.f ? 1.f : clip);  // (fminf would take a NaN for 1: no clipping)
+    }
   }
 };
 
@@ -601,6 +604,7 @@ extern "C" gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, cons
   args.correct2 = (float)(1.0 / sqrt(1.0 - pow(cfg->beta2, (double)cfg->step)));
   args.grad_scale = cfg->grad_scale;
   args.max_norm = (float)cfg->max_norm;
+  if (!isfinite(args.max_norm)) args.max_norm = 0.f;  // an infinite limit clips nothing
   args.key = mix32((uint32_t)cfg->step * 0x9E3779B9u + (uint32_t)cfg->seed);
   args.partial = a->d_partial;
   args.arrived = a->d_arrived;

@@ -481,7 +481,10 @@ typedef struct {
 } gz_adamw_tensor;
 typedef struct {
   double lr, beta1, beta2, eps;
-  double max_norm;       /* > 0: gradients are scaled down to this global norm */
+  double max_norm;       /* > 0: gradients are scaled down to this global norm: by
+                            max_norm / (norm + 1e-6) where that is below 1.  A norm
+                            of NaN makes every gradient NaN, an infinite one scales
+                            the finite gradients to 0.  Infinity: no clipping */
   float grad_scale;      /* factor on every gradient (1 / the loss scale, say) */
   int64_t step;          /* t, from 1 */
   uint64_t seed;         /* of the 8-bit rounding */

@@ -1,10 +1,11 @@
 """AdamW: its states' types, gradients and norms that are not finite, captures
 replayed, and tensors that have moved."""
+import numpy as np
 import pytest
 import torch
 
 import graphzero_b200 as gz
-from test_adamw_gpu import gradients, make
+from test_adamw_gpu import U, gradients, make
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +87,45 @@ def test_states_are_restored_in_place(cuda, bits):
         opt.params = weights
     with pytest.raises(TypeError):
         opt.params[0] = weights[0]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("many", [False, True])
+def test_clipping_by_a_norm_that_is_not_finite(cuda, bits, many):
+    """A NaN among the gradients makes every clipped gradient, and so every
+    weight that has one, NaN; an infinity alone scales the finite ones to 0
+    (and itself to NaN)."""
+    shapes = [(300, 3), (17,), (256,)] + [(5,)] * (900 if many else 0)
+    gs = gradients(shapes, 1)
+    gs[2] = None
+    gs[1][4] = float("nan")
+    params = make(shapes)
+    before = params[2].clone()
+    norm = gz.AdamW(params, state_bits=bits, max_norm=1.0).step(gs)
+    assert norm.isnan()
+    assert all(p.isnan().all() for k, p in enumerate(params) if k != 2) and torch.equal(params[2], before)
+
+    gs[1][4] = float("inf")
+    params, still = make(shapes), make(shapes)
+    norm = gz.AdamW(params, state_bits=bits, max_norm=1.0).step(gs)
+    assert float(norm) == float("inf")
+    gz.AdamW(still, state_bits=bits).step([None if g is None else torch.zeros_like(g) for g in gs])
+    assert params[1][4].isnan()
+    params[1][4] = still[1][4]
+    assert all(torch.equal(p, q) for p, q in zip(params, still))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_infinite_limit_only_measures_the_norm(cuda, bits):
+    shapes = [(300, 3), (17,)]
+    gs = gradients(shapes, 1)
+    for bad in (None, float("inf")):
+        if bad:
+            gs[1][4] = bad
+        a, b = make(shapes), make(shapes)
+        norm = gz.AdamW(a, state_bits=bits, max_norm=float("inf")).step(gs)
+        gz.AdamW(b, state_bits=bits).step(gs)
+        want = float(torch.sqrt(sum((g.double() ** 2).sum() for g in gs)))
+        assert float(norm) == want if bad else abs(float(norm) - want) <= 2 * U * want
+        for p, q in zip(a, b):
+            np.testing.assert_array_equal(p.cpu().numpy(), q.cpu().numpy())
