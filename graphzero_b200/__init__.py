@@ -168,6 +168,8 @@ _SIGS = {
     "gz_adamw_create": (C.c_int, [C.POINTER(AdamWTensor), C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
     "gz_adamw_destroy": (C.c_int, [_vp]),
     "gz_adamw_step": (C.c_int, [_vp, C.POINTER(_vp), _i32p, C.POINTER(AdamWConfig), _vp, _vp]),
+    "gz_adamw_get_steps": (C.c_int, [_vp, C.POINTER(C.c_int64)]),
+    "gz_adamw_set_steps": (C.c_int, [_vp, C.c_int64]),
     "gz_gat_c4_predict_noalloc": (C.c_int, [C.c_int, _f32p, C.c_size_t, _i8p, _i8p, C.c_int, _f32p, _f32p]),
     "gz_gat_c4_noalloc_scratch_bytes": (C.c_size_t, []),
     "gz_gat_c4_noalloc_max_batch": (C.c_int, []),
@@ -866,7 +868,12 @@ class AdamW:
     save; restore them in place (opt.m.copy_(saved), opt.steps = n).  The
     kernels hold the addresses of weights, copies and states: a step raises if
     one of them has moved to other memory (p.data = ..., a module moved between
-    devices).  `lr` and `max_norm` may be changed between steps."""
+    devices).  `lr` and `max_norm` may be changed between steps.
+
+    A step can be captured in a CUDA graph; every replay is then a step with the
+    next t, on the gradients at the captured addresses, with the capture's lr
+    and other settings.  `steps` counts replays too: it is read from the device
+    once a step has been captured, and reading it waits for the device then."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, copies=None,
                  lr_scale=1.0, max_norm=0.0, seed=0):
@@ -889,7 +896,8 @@ class AdamW:
             if c is not None and (c.dtype not in (torch.float16, torch.bfloat16) or c.shape != p.shape
                                   or c.device != self.device or not c.is_contiguous()):
                 raise ValueError("copies must be contiguous float16 or bfloat16 tensors of their weights' shapes")
-        self.lr, self.betas, self.eps, self.max_norm, self.seed, self.steps = lr, tuple(betas), eps, max_norm, seed, 0
+        self.lr, self.betas, self.eps, self.max_norm, self.seed = lr, tuple(betas), eps, max_norm, seed
+        self._steps, self._counted = 0, False  # whether t is the device's to count
         self.offsets, total = [], 0
         for p in self.params:
             self.offsets.append(total)
@@ -924,6 +932,19 @@ class AdamW:
     v = property(lambda self: self._v)
     m_scale = property(lambda self: self._m_scale)
     v_scale = property(lambda self: self._v_scale)
+
+    @property
+    def steps(self):
+        if not self._counted:
+            return self._steps
+        n = C.c_int64()
+        _check(_lib.gz_adamw_get_steps(self._plan, C.byref(n)))
+        return n.value
+
+    @steps.setter
+    def steps(self, n):
+        _check(_lib.gz_adamw_set_steps(self._plan, n))
+        self._steps = n
 
     def close(self) -> None:
         if self._plan:
@@ -968,10 +989,13 @@ class AdamW:
         norm = _torch.empty((), dtype=_torch.float32, device=self.device) if self.max_norm > 0 else None
         c = self._cfg
         c.lr, (c.beta1, c.beta2), c.eps = self.lr, self.betas, self.eps
-        c.max_norm, c.grad_scale, c.step, c.seed = self.max_norm, grad_scale, self.steps + 1, self.seed
+        if _torch._C._cuda_isCurrentStreamCapturing():
+            self._counted = True  # from here on replays may come between
+        c.max_norm, c.grad_scale, c.seed = self.max_norm, grad_scale, self.seed
+        c.step = 0 if self._counted else self._steps + 1
         _check(_lib.gz_adamw_step(self._plan, self._grads, self._kinds, C.byref(c), norm if norm is None else norm.data_ptr(),
                                   _current_stream(self.device)))
-        self.steps += 1
+        self._steps += 1
         return norm
 
 

@@ -4,7 +4,10 @@
 // A plan cuts every tensor into chunks of whole 256-element blocks and keeps
 // the tensors' table and the chunk list on the device; a step launches one
 // block of threads per chunk.  The gradients' addresses change from step to
-// step, so they travel as kernel arguments.
+// step, so they travel as kernel arguments.  So does what depends on the step's
+// number t, worked out by the host; a step that is captured to be replayed
+// counts on the device instead, where a kernel of one thread works the same out
+// before the others.
 //
 // Every operation of the update is rounded by itself (no contraction), so a
 // step reproduces an elementwise evaluation of the formulas bit for bit; that
@@ -52,15 +55,30 @@ struct Grads {
   uint8_t dtype[kGradsPerLaunch];
 };
 
+// What depends on the step's number t.
+struct Timed {
+  double lr_corrected;  // lr / (1 - beta1^t)
+  float correct2;       // 1 / sqrt(1 - beta2^t)
+  uint32_t key;         // of the rounding
+};
+
+// t as the device counts it, and what depends on it in a counted step.
+struct Count {
+  int64_t t;
+  Timed timed;
+};
+
 struct StepArgs {
   const Tensor* tensors;
   const Chunk* chunks;     // of this launch
   int first_tensor;        // grads.p[0] belongs to it
   uint32_t blocks;         // blocks per chunk
-  double lr, lr_corrected;  // lr, lr / (1 - beta1^t)
-  float beta1, one_beta1, beta2, one_beta2, eps, correct2;  // correct2 = 1 / sqrt(1 - beta2^t)
+  double lr;
+  float beta1, one_beta1, beta2, one_beta2, eps;
   float grad_scale, max_norm;  // max_norm 0: no clipping
-  uint32_t key;            // of the rounding
+  int64_t t;               // of a step that is not counted on the device
+  Timed timed;
+  Count* count;
   double* partial;         // sums of squares, one per chunk of the plan
   unsigned* arrived;
   int chunk_base, chunk_count;  // first chunk of this launch, chunks of the plan
@@ -266,12 +284,28 @@ template <int kBits> struct Raw {
   }
 };
 
+__host__ __device__ inline Timed timed_at(int64_t t, double lr, double beta1, double beta2, uint32_t seed) {
+  return {lr / (1.0 - pow(beta1, (double)t)), (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))),
+          mix32((uint32_t)t * 0x9E3779B9u + seed)};
+}
+
+// One thread: the step's number where the host has not given it (t = 0).
+__global__ void count_kernel(Count* count, int64_t t, double lr, double beta1, double beta2, uint32_t seed) {
+  if (t == 0) t = count->t + 1;
+  count->t = t;
+  count->timed = timed_at(t, lr, beta1, beta2, seed);
+}
+
 // The numbers of a step that a chunk's tensor goes by.
-struct Rates {
-  float decay, step, scale;
+template <bool kCounted> struct Rates {
+  float decay, step, scale, correct2;
+  uint32_t key;
   __device__ Rates(const StepArgs& a, const Tensor& t) {
+    const Timed& timed = kCounted ? a.count->timed : a.timed;
+    correct2 = timed.correct2;
+    key = timed.key;
     decay = (float)(1.0 - a.lr * t.lr_scale * t.weight_decay);
-    step = (float)(a.lr_corrected * t.lr_scale);
+    step = (float)(timed.lr_corrected * t.lr_scale);
     scale = a.grad_scale;
     if (a.max_norm > 0.f) {
       const float clip = __fdiv_rn(a.max_norm, __fadd_rn(*a.norm, 1e-6f));
@@ -282,8 +316,8 @@ struct Rates {
 
 // The update of a lane's elements; v holds the root of the second moment going
 // in with 8-bit states, and root the new one's.
-template <int kBits>
-__device__ __forceinline__ void update(const StepArgs& a, const Rates& rate, float* x, float* p, float* m, float* v, float* root) {
+template <int kBits, bool kCounted>
+__device__ __forceinline__ void update(const StepArgs& a, const Rates<kCounted>& rate, float* x, float* p, float* m, float* v, float* root) {
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
     if (kBits == 8) v[k] = __fmul_rn(v[k], v[k]);
@@ -291,19 +325,19 @@ __device__ __forceinline__ void update(const StepArgs& a, const Rates& rate, flo
     m[k] = __fadd_rn(__fmul_rn(m[k], a.beta1), __fmul_rn(x[k], a.one_beta1));
     v[k] = __fadd_rn(__fmul_rn(v[k], a.beta2), __fmul_rn(__fmul_rn(x[k], x[k]), a.one_beta2));
     root[k] = __fsqrt_rn(v[k]);
-    const float move = __fdiv_rn(m[k], __fadd_rn(__fmul_rn(root[k], a.correct2), a.eps));
+    const float move = __fdiv_rn(m[k], __fadd_rn(__fmul_rn(root[k], rate.correct2), a.eps));
     p[k] = __fsub_rn(__fmul_rn(p[k], rate.decay), __fmul_rn(move, rate.step));
   }
 }
 
 // Rounds a block's new states to 8 bits and stores them.
-__device__ __forceinline__ void store_8bit(const StepArgs& a, const Tensor& t, uint32_t block, int lane, float* m, float* root) {
+__device__ __forceinline__ void store_8bit(uint32_t key, const Tensor& t, uint32_t block, int lane, float* m, float* root) {
   const int64_t at = (int64_t)block * kBlock;
   const float m_most = warp_most(m), v_most = warp_most(root);
   const int me = scale_exponent(fabsf(m_most)), ve = scale_exponent(fabsf(v_most));
   const float m_down = power(-me), v_down = power(-ve);
   const bool odd = signbit(m_most) || signbit(v_most);  // something is not finite
-  const uint32_t first = (uint32_t)(t.first + at) + lane * kRun + a.key;
+  const uint32_t first = (uint32_t)(t.first + at) + lane * kRun + key;
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
     const uint32_t h = mix32(first + place(0, k));
@@ -331,10 +365,10 @@ __device__ __forceinline__ void store_8bit(const StepArgs& a, const Tensor& t, u
 }
 
 // A block at a tensor's end, or of one that is not aligned: element by element.
-template <int kBits>
+template <int kBits, bool kCounted>
 __device__ __noinline__ void step_ragged(const StepArgs& a, const Tensor* tensor, const void* g, int dtype, uint32_t block, int lane) {
   const Tensor t = *tensor;
-  const Rates rate(a, t);
+  const Rates<kCounted> rate(a, t);
   const int64_t at = (int64_t)block * kBlock;
   float x[kPerLane], p[kPerLane], m[kPerLane], v[kPerLane], root[kPerLane];
   const float ms = kBits == 8 ? t.m_scale[block] : 1.f, vs = kBits == 8 ? t.v_scale[block] : 1.f;
@@ -359,7 +393,7 @@ __device__ __noinline__ void step_ragged(const StepArgs& a, const Tensor* tensor
       v[k] = in ? __fmul_rn(v[k], vs) : 0.f;
     }
   }
-  update<kBits>(a, rate, x, p, m, v, root);
+  update<kBits, kCounted>(a, rate, x, p, m, v, root);
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
     const int64_t i = at + place(lane, k);
@@ -374,21 +408,22 @@ __device__ __noinline__ void step_ragged(const StepArgs& a, const Tensor* tensor
       else ((__nv_bfloat16*)t.copy)[i] = __float2bfloat16_rn(p[k]);
     }
   }
-  if (kBits == 8) store_8bit(a, t, block, lane, m, root);
+  if (kBits == 8) store_8bit(rate.key, t, block, lane, m, root);
 }
 
 // A warp per 256-element block, several in turn; with 8-bit states the next
 // block is read while one is worked on.  Every array is read and written once,
 // past the caches (nothing is used again within the step): bound by memory.
-template <int kBits>
+template <int kBits, bool kCounted>
 __global__ void __launch_bounds__(kThreads, kStepBlocks) step_kernel(const __grid_constant__ StepArgs a, const __grid_constant__ Grads grads) {
   const Chunk c = a.chunks[blockIdx.x];
   const Tensor t = a.tensors[c.tensor];
   const void* g = grads.p[c.tensor - a.first_tensor];
   const int dtype = grads.dtype[c.tensor - a.first_tensor];
+  if (!kCounted && blockIdx.x == 0 && threadIdx.x == 0) a.count->t = a.t;  // for a counted step after this one
   if (!g) return;
   const int lane = threadIdx.x % 32;
-  const Rates rate(a, t);
+  const Rates<kCounted> rate(a, t);
   bool aligned = grads_aligned(g, dtype) && ((uintptr_t)t.param & 15) == 0 && ((uintptr_t)t.copy & 7) == 0;
   if (kBits == 32) aligned = aligned && (((uintptr_t)t.m | (uintptr_t)t.v) & 15) == 0;
   const uint32_t end = min((uint32_t)((t.n + kBlock - 1) / kBlock), c.block + a.blocks);
@@ -418,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, kStepBlocks) step_kernel(const __gri
         }
       }
     }
-    update<kBits>(a, rate, x, p, m, v, root);
+    update<kBits, kCounted>(a, rate, x, p, m, v, root);
 #pragma unroll
     for (int k = 0; k < kPerLane; k += kRun) {
       const int64_t i = (int64_t)b * kBlock + place(lane, k);
@@ -439,10 +474,10 @@ __global__ void __launch_bounds__(kThreads, kStepBlocks) step_kernel(const __gri
         __stcs((uint2*)((uint16_t*)t.copy + i), raw);
       }
     }
-    if (kBits == 8) store_8bit(a, t, b, lane, m, root);
+    if (kBits == 8) store_8bit(rate.key, t, b, lane, m, root);
     else if (b + kThreads / 32 < whole) next.load(t, g, dtype, b + kThreads / 32, lane);
   }
-  for (; b < end; b += kThreads / 32) step_ragged<kBits>(a, a.tensors + c.tensor, g, dtype, b, lane);
+  for (; b < end; b += kThreads / 32) step_ragged<kBits, kCounted>(a, a.tensors + c.tensor, g, dtype, b, lane);
 }
 
 }  // namespace
@@ -453,10 +488,11 @@ using namespace gz;
 struct gz_adamw {
   int device = 0, state_bits = 32, count = 0;
   uint32_t blocks_per_chunk = 0;
-  void* arena = nullptr;  // tensors | chunks | partial sums | counter and norm
+  void* arena = nullptr;  // tensors | chunks | partial sums | count, norm and counter of blocks
   Tensor* d_tensors = nullptr;
   Chunk* d_chunks = nullptr;
   double* d_partial = nullptr;
+  Count* d_count = nullptr;
   unsigned* d_arrived = nullptr;
   float* d_norm = nullptr;
   std::vector<int> chunk_start;  // per tensor, and the total
@@ -532,9 +568,11 @@ gz_status create(const gz_adamw_tensor* tensors, int count, int state_bits, int 
   a->d_tensors = (Tensor*)p;
   a->d_chunks = (Chunk*)(p + tb);
   a->d_partial = (double*)(p + tb + cb);
-  a->d_arrived = (unsigned*)(p + tb + cb + pb);
-  a->d_norm = (float*)(a->d_arrived + 1);
-  cudaError_t e = cudaMemset(a->d_arrived, 0, 256);
+  a->d_count = (Count*)(p + tb + cb + pb);
+  a->d_norm = (float*)(a->d_count + 1);
+  a->d_arrived = (unsigned*)(a->d_norm + 1);
+  static_assert(sizeof(Count) + 8 <= 256, "they fit the arena's end");
+  cudaError_t e = cudaMemset(a->d_count, 0, 256);
   if (e == cudaSuccess && count) e = cudaMemcpy(a->d_tensors, table.data(), sizeof(Tensor) * table.size(), cudaMemcpyHostToDevice);
   if (e == cudaSuccess && !chunks.empty())
     e = cudaMemcpy(a->d_chunks, chunks.data(), sizeof(Chunk) * chunks.size(), cudaMemcpyHostToDevice);
@@ -585,7 +623,7 @@ extern "C" gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, cons
   if (!(cfg->beta1 >= 0 && cfg->beta1 < 1) || !(cfg->beta2 >= 0 && cfg->beta2 < 1)) return bad(who, "betas must be in [0, 1)");
   if (!(cfg->eps >= 0) || !isfinite(cfg->eps)) return bad(who, "eps must be finite and at least 0");
   if (!(cfg->max_norm >= 0)) return bad(who, "max_norm must be at least 0");
-  if (cfg->step < 1) return bad(who, "steps count from 1");
+  if (cfg->step < 0) return bad(who, "steps count from 1 (0: counted on the device)");
   for (int k = 0; grad_dtypes && k < a->count; ++k)
     if (grad_dtypes[k] < GZ_F32 || grad_dtypes[k] > GZ_BF16) return bad(who, "bad gradient dtype");
   Device on(a->device);
@@ -595,21 +633,26 @@ extern "C" gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, cons
   args.tensors = a->d_tensors;
   args.blocks = a->blocks_per_chunk;
   args.lr = cfg->lr;
-  args.lr_corrected = cfg->lr / (1.0 - pow(cfg->beta1, (double)cfg->step));
   args.beta1 = (float)cfg->beta1;
   args.one_beta1 = (float)(1.0 - cfg->beta1);
   args.beta2 = (float)cfg->beta2;
   args.one_beta2 = (float)(1.0 - cfg->beta2);
   args.eps = (float)cfg->eps;
-  args.correct2 = (float)(1.0 / sqrt(1.0 - pow(cfg->beta2, (double)cfg->step)));
   args.grad_scale = cfg->grad_scale;
   args.max_norm = (float)cfg->max_norm;
   if (!isfinite(args.max_norm)) args.max_norm = 0.f;  // an infinite limit clips nothing
-  args.key = mix32((uint32_t)cfg->step * 0x9E3779B9u + (uint32_t)cfg->seed);
+  const bool counted = cfg->step == 0;
+  args.t = cfg->step;
+  args.count = a->d_count;
+  if (!counted) args.timed = timed_at(cfg->step, cfg->lr, cfg->beta1, cfg->beta2, (uint32_t)cfg->seed);
   args.partial = a->d_partial;
   args.arrived = a->d_arrived;
   args.chunk_count = a->chunk_start.back();
   args.norm = d_norm ? d_norm : a->d_norm;
+  if (counted || args.chunk_count == 0) {
+    count_kernel<<<1, 1, 0, s>>>(a->d_count, cfg->step, cfg->lr, cfg->beta1, cfg->beta2, (uint32_t)cfg->seed);
+    if (cudaError_t e = cudaGetLastError()) return cuda_failed(who, e);
+  }
   if (d_norm && args.chunk_count == 0)
     if (cudaError_t e = cudaMemsetAsync(d_norm, 0, sizeof(float), s)) return cuda_failed(who, e);
   Grads g;
@@ -626,9 +669,31 @@ extern "C" gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, cons
       args.chunks = a->d_chunks + base;
       args.chunk_base = base;
       if (pass == 0) norm_kernel<<<n, kThreads, 0, s>>>(args, g);
-      else if (a->state_bits == 8) step_kernel<8><<<n, kThreads, 0, s>>>(args, g);
-      else step_kernel<32><<<n, kThreads, 0, s>>>(args, g);
+      else if (a->state_bits == 8) (counted ? step_kernel<8, true> : step_kernel<8, false>)<<<n, kThreads, 0, s>>>(args, g);
+      else (counted ? step_kernel<32, true> : step_kernel<32, false>)<<<n, kThreads, 0, s>>>(args, g);
       if (cudaError_t e = cudaGetLastError()) return cuda_failed(who, e);
     }
   return GZ_OK;
+}
+
+extern "C" gz_status gz_adamw_get_steps(gz_adamw* a, int64_t* steps) {
+  const char* who = "gz_adamw_get_steps";
+  if (!a || !steps) return bad(who, "null argument");
+  Device on(a->device);
+  if (!on.ok) return set_last_error(GZ_ERR_CUDA, "%s: cannot select CUDA device %d", who, a->device);
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(steps, &a->d_count->t, sizeof(int64_t), cudaMemcpyDeviceToHost);
+  return e == cudaSuccess ? GZ_OK : cuda_failed(who, e);
+}
+
+extern "C" gz_status gz_adamw_set_steps(gz_adamw* a, int64_t steps) {
+  const char* who = "gz_adamw_set_steps";
+  if (!a) return bad(who, "null argument");
+  if (steps < 0) return bad(who, "steps must be at least 0");
+  Device on(a->device);
+  if (!on.ok) return set_last_error(GZ_ERR_CUDA, "%s: cannot select CUDA device %d", who, a->device);
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(&a->d_count->t, &steps, sizeof(int64_t), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  return e == cudaSuccess ? GZ_OK : cuda_failed(who, e);
 }

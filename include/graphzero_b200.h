@@ -486,8 +486,9 @@ typedef struct {
                             of NaN makes every gradient NaN, an infinite one scales
                             the finite gradients to 0.  Infinity: no clipping */
   float grad_scale;      /* factor on every gradient (1 / the loss scale, say) */
-  int64_t step;          /* t, from 1 */
-  uint64_t seed;         /* of the 8-bit rounding */
+  int64_t step;          /* t, from 1; 0: one more than the plan's last step, counted on
+                            the device */
+  uint64_t seed;         /* of the 8-bit rounding (its lower 32 bits) */
 } gz_adamw_config;
 typedef struct gz_adamw gz_adamw;
 /* A plan over `count` tensors of `device` (host array; the buffers stay the
@@ -499,9 +500,18 @@ gz_status gz_adamw_destroy(gz_adamw* a);
  * host array of their gz_dtype, NULL: all GZ_F32.  d_norm (may be NULL; one
  * float on the device) receives the global 2-norm of the scaled gradients.
  * The norm is taken when max_norm > 0 or d_norm is given, in a fixed order.
- * Steps of one plan must be ordered (one stream, or events between them). */
+ * Steps of one plan must be ordered (one stream, or events between them).
+ * In a graph the call's arguments stay those of the capture, the addresses of
+ * the gradients among them.  With cfg->step 0 every replay is a step of its own:
+ * t, and with it the bias corrections and the rounding numbers, goes on from
+ * wherever calls and replays before it have left it.  (With another cfg->step
+ * every replay repeats that t.) */
 gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, const int32_t* grad_dtypes,
                         const gz_adamw_config* cfg, float* d_norm, void* stream);
+/* The number t of the plan's last step (0 before the first), and setting it (a
+ * restored run's).  Both synchronise the device, and neither can be captured. */
+gz_status gz_adamw_get_steps(gz_adamw* a, int64_t* steps);
+gz_status gz_adamw_set_steps(gz_adamw* a, int64_t steps);
 
 /* ---- allocation-free leaf evaluation --------------------------------------
  * No counterpart in the reference.  For callers that may not allocate device

@@ -129,3 +129,101 @@ def test_an_infinite_limit_only_measures_the_norm(cuda, bits):
         assert float(norm) == want if bad else abs(float(norm) - want) <= 2 * U * want
         for p, q in zip(a, b):
             np.testing.assert_array_equal(p.cpu().numpy(), q.cpu().numpy())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("max_norm", [0.0, 0.01])
+def test_replays_of_a_capture_are_steps(cuda, bits, max_norm):
+    """Calls, replays and calls again are the same steps as as many calls: bias
+    corrections, rounding numbers and the count go on from wherever they are."""
+    shapes = [(500, 20), (33,)]
+    a, b = make(shapes), make(shapes)
+    kw = dict(state_bits=bits, max_norm=max_norm, lr=1e-2, betas=(0.8, 0.95), seed=3)
+    x, y = gz.AdamW(a, **kw), gz.AdamW(b, **kw)
+    gs = gradients(shapes, 0)
+
+    def new_gradients(t):
+        for g, h in zip(gs, gradients(shapes, 10 + t)):
+            g.copy_(h)
+
+    t = 0
+    for _ in range(2):
+        new_gradients(t)
+        x.step(gs), y.step(gs)
+        t += 1
+    assert x.steps == y.steps == 2
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = y.step(gs)
+    assert y.steps == 2  # a capture is not a step
+    for _ in range(4):
+        new_gradients(t)
+        n = x.step(gs)
+        graph.replay()
+        t += 1
+        assert norm is None or torch.equal(n, norm)
+    assert x.steps == y.steps == t == 6
+    for _ in range(2):
+        new_gradients(t)
+        x.step(gs), y.step(gs)
+        t += 1
+    new_gradients(t)
+    x.step(gs)
+    graph.replay()
+    assert x.steps == y.steps == 9
+    # restored to another place
+    x.steps = y.steps = 100
+    new_gradients(t)
+    x.step(gs)
+    graph.replay()
+    assert x.steps == y.steps == 101
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert torch.equal(x.m.float(), y.m.float()) and torch.equal(x.v.float(), y.v.float())
+
+
+def test_a_restored_count_is_where_a_capture_starts(cuda):
+    a, b = make([(700,)]), make([(700,)])
+    x, y = gz.AdamW(a, state_bits=8), gz.AdamW(b, state_bits=8)
+    gs = gradients([(700,)], 2)
+    x.steps = y.steps = 40
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y.step(gs)
+    for _ in range(3):
+        x.step(gs)
+        graph.replay()
+    assert x.steps == y.steps == 43
+    assert torch.equal(a[0], b[0]) and torch.equal(x.v.float(), y.v.float())
+
+
+def test_capture_of_a_plan_in_several_launches(cuda):
+    shapes = [(k % 37 + 1, 11) for k in range(1000)] + [(0,)]
+    a, b, gs = make(shapes), make(shapes), gradients(shapes, 7)
+    gs[999] = gs[0] = None
+    x, y = gz.AdamW(a, state_bits=8, max_norm=0.3), gz.AdamW(b, state_bits=8, max_norm=0.3)
+    x.step(gs), y.step(gs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y.step(gs)
+    for _ in range(3):
+        x.step(gs)
+        graph.replay()
+    assert x.steps == y.steps == 4
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_steps_of_a_plan_without_gradients_count(cuda):
+    p = make([(9,)])
+    opt = gz.AdamW(p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step([None])
+    graph.replay()
+    graph.replay()
+    assert opt.steps == 2
+    opt.step([None])
+    assert opt.steps == 3
+    for bad in (-1, 2**63):
+        with pytest.raises((ValueError, gz.GZError)):
+            opt.steps = bad
+    assert opt.steps == 3
