@@ -154,6 +154,7 @@ _SIGS = {
     "gz_train_examples_load": (C.c_int, [C.c_char_p, _vp, C.c_int64, _i32p, C.c_int, C.POINTER(C.c_int),
                                          C.POINTER(C.c_int64)]),
     "gz_selftest_wait_timeout": (C.c_int, [C.c_int, C.c_int]),
+    "gz_selftest_cluster_wait_timeout": (C.c_int, [C.c_int, C.c_int]),
     "gz_train_config_default": (None, [C.POINTER(TrainConfig)]),
     "gz_net_loss_grad": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, _vp, _f32p, _vp]),
     "gz_net_train_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, C.POINTER(TrainConfig), _vp, C.c_int, _f32p,
@@ -234,6 +235,12 @@ def selftest_wait_timeout(device: int = 0, limit_us: int = 20000) -> int:
     """Status of a kernel whose bounded wait on a never-arriving barrier runs
     out (GZ_ERR_TIMEOUT expected; the context stays usable)."""
     return int(_lib.gz_selftest_wait_timeout(device, limit_us))
+
+
+def selftest_cluster_wait_timeout(device: int = 0, limit_us: int = 20000) -> int:
+    """The same for blocks that share a row in policy_loss and wait for each
+    other's sums: GZ_ERR_TIMEOUT where the waits ran out and left NaN."""
+    return int(_lib.gz_selftest_cluster_wait_timeout(device, limit_us))
 
 
 def version() -> str:

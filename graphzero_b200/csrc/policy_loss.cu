@@ -304,13 +304,15 @@ struct LossShared {
   int counts[kListedThreads / 32];
   alignas(16) Part inbox[2][kMostSlices];  // the cluster's parts, the block's rows in turn
   uint64_t filled[2];
+  int gave_up;
 };
 
 // The cluster's blocks send each other their parts: 16 bytes each into every
 // inbox, whose barrier counts the bytes; nobody waits for another's copies.
-__device__ __forceinline__ void open_inbox(const LossArgs& a, LossShared& sh) {
-  if (a.cluster == 1) return;
+__device__ __forceinline__ void open_inbox(int cluster, LossShared& sh) {
+  if (cluster == 1) return;
   if (threadIdx.x == 0) {
+    sh.gave_up = 0;
     sm100::mbar_init(&sh.filled[0], 1);
     sm100::mbar_init(&sh.filled[1], 1);
     sm100::fence_mbar_init();
@@ -321,25 +323,34 @@ __device__ __forceinline__ void open_inbox(const LossArgs& a, LossShared& sh) {
 __device__ __forceinline__ void wait_cluster() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // All blocks' parts, joined in the blocks' order, for the block's row number
-// `turn`.  A block is at most one row ahead of the others (it needs their
-// parts), so two inboxes in turn never mix.
-__device__ __forceinline__ Part exchange(Part p, const LossArgs& a, int rank, unsigned turn, LossShared& sh) {
-  Part* inbox = sh.inbox[turn & 1];
+// `turn`, once all are there.  A wait that lasts longer than `limit_ns` gives
+// up: its thread gets a NaN for every sum, and its block for all rows after
+// this one, without sending or waiting again (the others, then short of its
+// parts, give up in their turn).  So what is written is right or NaN, a program
+// loses a few waits at most, and no inbox gets a part of another row's.
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+
+__device__ __forceinline__ Part no_part() { return {NAN, NAN, NAN, NAN}; }
+__device__ __forceinline__ bool gave_up(const LossShared& sh) { return *(const volatile int*)&sh.gave_up; }
+
+__device__ __forceinline__ void send_part(Part p, int cluster, int rank, unsigned turn, LossShared& sh) {
+  if (threadIdx.x >= cluster) return;
+  uint32_t to, bar;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sm100::smem_u32(&sh.inbox[turn & 1][rank])), "r"(threadIdx.x));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(sm100::smem_u32(&sh.filled[turn & 1])), "r"(threadIdx.x));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+               "r"(__float_as_uint(p.m)), "r"(__float_as_uint(p.z)), "r"(__float_as_uint(p.mass)),
+               "r"(__float_as_uint(p.cross)), "r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ Part receive_parts(int cluster, unsigned turn, LossShared& sh, uint64_t limit_ns) {
+  const Part* inbox = sh.inbox[turn & 1];
   uint64_t* filled = &sh.filled[turn & 1];
-  if (turn == 0) wait_cluster();  // every inbox is open
-  if (threadIdx.x < a.cluster) {
-    uint32_t to, bar;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sm100::smem_u32(&inbox[rank])), "r"(threadIdx.x));
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(sm100::smem_u32(filled)), "r"(threadIdx.x));
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
-                 "r"(__float_as_uint(p.m)), "r"(__float_as_uint(p.z)), "r"(__float_as_uint(p.mass)),
-                 "r"(__float_as_uint(p.cross)), "r"(bar)
-                 : "memory");
-    if (threadIdx.x == 0) sm100::mbar_arrive_expect_tx(filled, a.cluster * sizeof(Part));
-  }
+  if (threadIdx.x == 0) sm100::mbar_arrive_expect_tx(filled, cluster * sizeof(Part));
   const uint64_t began = sm100::global_timer_ns();
   uint32_t done = 0;
-  while (!done) {  // gives up after 4 s: what is not filled then makes the row wrong, not the program hang
+  while (!done) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
@@ -347,11 +358,23 @@ __device__ __forceinline__ Part exchange(Part p, const LossArgs& a, int rank, un
         : "=r"(done)
         : "r"(sm100::smem_u32(filled)), "r"(turn >> 1 & 1)
         : "memory");
-    if (!done && sm100::global_timer_ns() - began > 4000000000ull) break;
+    if (!done && sm100::global_timer_ns() - began > limit_ns) {
+      *(volatile int*)&sh.gave_up = 1;
+      return no_part();
+    }
   }
-  p = inbox[0];
-  for (int k = 1; k < a.cluster; ++k) p = merge(p, inbox[k]);
+  Part p = inbox[0];
+  for (int k = 1; k < cluster; ++k) p = merge(p, inbox[k]);
   return p;
+}
+
+// Both.  A block is at most one row ahead of the others (it needs their parts),
+// so two inboxes in turn never mix.
+__device__ __forceinline__ Part exchange(Part p, int cluster, int rank, unsigned turn, LossShared& sh) {
+  if (turn == 0) wait_cluster();  // every inbox is open
+  if (gave_up(sh)) return no_part();
+  send_part(p, cluster, rank, turn, sh);
+  return receive_parts(cluster, turn, sh, kWaitLimitNs);
 }
 
 // Maximum over the block.
@@ -399,14 +422,14 @@ __device__ __forceinline__ Part block_merge(Part p, Part* slots) {
 template <bool kDense>
 __device__ __forceinline__ Result join(Part p, const LossArgs& a, int64_t row, int rank, unsigned turn, float weight,
                                        bool labelled, float label_x, LossShared& sh) {
-  if (a.cluster > 1) p = exchange(p, a, rank, turn, sh);
+  if (a.cluster > 1) p = exchange(p, a.cluster, rank, turn, sh);
   const Result q = result_of<kDense>(p, a.scale, weight, labelled, label_x);
   if (rank == 0 && threadIdx.x == 0) a.loss[row] = q.loss;
   return q;
 }
 // A block's shared memory stays until the others have sent what they send.
-__device__ __forceinline__ void leave(const LossArgs& a) {
-  if (a.cluster == 1) return;
+__device__ __forceinline__ void leave(int cluster) {
+  if (cluster == 1) return;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   wait_cluster();
 }
@@ -594,7 +617,7 @@ __global__ void __launch_bounds__(kLossThreads, 2) loss_kernel(const __grid_cons
   const int tid = threadIdx.x, n = blockDim.x, rank = blockIdx.x % a.cluster;
   const int64_t step = gridDim.x / a.cluster;
   int64_t row = a.first_row + blockIdx.x / a.cluster;
-  open_inbox(a, sh);
+  open_inbox(a.cluster, sh);
   LossRow<T> now(a, row, rank, kDense);
   now.vecs = 0;  // nothing to write yet
   Result q{Scale(0.f), 0.f, 0.f, 0.f};
@@ -655,19 +678,41 @@ __global__ void __launch_bounds__(kLossThreads, 2) loss_kernel(const __grid_cons
     now = next;
     row = next_row;
   }
-  leave(a);
+  leave(a.cluster);
 }
 
 template <typename T, bool kDense>
 __global__ void __launch_bounds__(kListedThreads, 8) loss_masked_kernel(const __grid_constant__ LossArgs a) {
   __shared__ LossShared sh;
   __shared__ __align__(8) int list[kListed * 3];
-  open_inbox(a, sh);
+  open_inbox(a.cluster, sh);
   if (!listed_slice<T, kDense>(a, list, sh)) {
     __syncthreads();
     masked_dense_slice<T, kDense>(a, sh);
   }
-  leave(a);
+  leave(a.cluster);
+}
+
+// Two blocks that wait for parts nobody sends.  *status: 1 where every thread's
+// first wait gave up, the next row was given up at once, and a row's loss and
+// gradient come out as NaN; else 0.
+__global__ void __cluster_dims__(2, 1, 1) wait_limit_kernel(uint64_t limit_ns, int* status) {
+  __shared__ LossShared sh;
+  open_inbox(2, sh);
+  wait_cluster();
+  Part p = receive_parts(2, 0, sh, limit_ns);
+  bool fine = p.z != p.z;
+  __syncthreads();
+  const uint64_t began = sm100::global_timer_ns();
+  p = exchange({0.f, 1.f, 1.f, 0.f}, 2, blockIdx.x, 1, sh);
+  fine = fine && p.z != p.z && sm100::global_timer_ns() - began < limit_ns;
+  const Result dense = result_of<true>(p, 1.f, 1.f, false, 0.f), label = result_of<false>(p, 1.f, 1.f, true, 0.f);
+  for (const Result& q : {dense, label}) {
+    const float grad = q.e(0.f) * q.share;
+    fine = fine && q.loss != q.loss && grad != grad;
+  }
+  if (!fine) atomicAnd(status, 0);
+  leave(2);
 }
 
 template <typename T, bool kDense>
@@ -756,4 +801,26 @@ extern "C" gz_status gz_policy_loss(const gz_policy_rows* rows, const float* d_t
   else if (rows->dtype == GZ_F16) e = d_target ? launch_loss<__half, true>(a, rows->rows, s) : launch_loss<__half, false>(a, rows->rows, s);
   else e = d_target ? launch_loss<__nv_bfloat16, true>(a, rows->rows, s) : launch_loss<__nv_bfloat16, false>(a, rows->rows, s);
   return e == cudaSuccess ? GZ_OK : set_last_error(GZ_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+extern "C" gz_status gz_selftest_cluster_wait_timeout(int device, int limit_us) {
+  const char* who = "gz_selftest_cluster_wait_timeout";
+  if (limit_us <= 0 || limit_us > 10000000) return bad(who, "limit_us out of range");
+  int before = 0, fine = 1;
+  int* status = nullptr;
+  cudaError_t e = cudaGetDevice(&before);
+  if (e == cudaSuccess) e = cudaSetDevice(device);
+  if (e != cudaSuccess) return set_last_error(GZ_ERR_CUDA, "%s: cannot select CUDA device %d", who, device);
+  e = cudaMalloc(&status, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemcpy(status, &fine, sizeof(int), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess) {
+    wait_limit_kernel<<<2, 64>>>(limit_us * 1000ull, status);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaMemcpy(&fine, status, sizeof(int), cudaMemcpyDeviceToHost);
+  cudaFree(status);
+  cudaSetDevice(before);
+  if (e != cudaSuccess) return set_last_error(GZ_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  if (!fine) return GZ_OK;
+  return set_last_error(GZ_ERR_TIMEOUT, "%s: bounded waits gave up after %d us and left NaN (expected)", who, limit_us);
 }

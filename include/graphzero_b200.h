@@ -448,7 +448,10 @@ gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sample_config* c
  * one of the two is given.  d_weight [rows] holds w (NULL: 1), an advantage
  * for instance.  A row without a visible score above -inf: loss 0, gradient
  * 0.  A NaN or +inf among the visible scores makes the row's loss and
- * gradient NaN.  d_loss [rows] fp32; d_grad [rows][actions] of the logits'
+ * gradient NaN.  Blocks that share a long row wait for each other's sums, for 4
+ * s at most; where one gives up, its part of the gradient (for the first block
+ * the loss too) is NaN in that row and in the rows that it would have done
+ * after it.  d_loss [rows] fp32; d_grad [rows][actions] of the logits'
  * dtype, NULL for the loss alone, and it overlaps no input.  fp32 inside,
  * in an order that depends on the row's length and alignment only. */
 gz_status gz_policy_loss(const gz_policy_rows* rows, const float* d_target, int64_t target_stride,
@@ -546,6 +549,11 @@ int gz_gat_c4_noalloc_max_batch(void);
  * GZ_OK if it somehow completed, GZ_ERR_CUDA on a launch error.  The CUDA
  * context stays usable afterwards. */
 gz_status gz_selftest_wait_timeout(int device, int limit_us);
+/* The same for the wait of blocks that share a row in gz_policy_loss: two blocks
+ * wait for sums that are never sent.  GZ_ERR_TIMEOUT when every wait gave up and
+ * the row's results are NaN, which is what a row then gets (the expected
+ * outcome), GZ_OK if not, GZ_ERR_CUDA on an error. */
+gz_status gz_selftest_cluster_wait_timeout(int device, int limit_us);
 
 #ifdef __cplusplus
 }

@@ -103,3 +103,11 @@ def test_loss_of_scores_of_any_magnitude(cuda, n, a, share, dtype):
         p = np.abs(wgrad + amount) + amount
         bound = 25 * few * p + half * np.abs(wgrad) + least + 2.0**-64
         assert (np.abs(grad.float().cpu().numpy() - wgrad) <= bound).all()
+
+
+def test_a_wait_that_runs_out_leaves_nan(cuda):
+    """Blocks that share a row wait for sums that nothing sends: the waits give
+    up after their limit, the results are NaN, and the next call is right."""
+    assert gz.selftest_cluster_wait_timeout(0, 20000) == gz.ERR_TIMEOUT
+    assert gz.selftest_cluster_wait_timeout(0, 0) == gz.ERR_INVALID_ARG
+    check_loss(rows_of(3, 60000, 1), label=torch.arange(3, dtype=torch.int32))
