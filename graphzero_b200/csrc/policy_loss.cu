@@ -22,6 +22,7 @@ struct LossArgs {
 constexpr int64_t kRowsPerLaunch = 1 << 26;  // rows x 16 blocks stay a valid grid
 constexpr int kSharedPerSM = 227 * 1024;
 constexpr int kSliceVecs = 6400;             // 16-byte vectors of a block's slice of a row: two blocks fit an SM
+constexpr int kMostScores = (kSliceVecs + 8) * 16;  // bytes of a slice, its end rounded up to 16 actions
 
 // What a part of a row contributes: m the largest visible score, z the sum of
 // exp(x - m), mass and cross the sums of t and t (x - m).  With m = -inf
@@ -741,8 +742,10 @@ cudaError_t launch_loss(LossArgs a, int64_t rows, cudaStream_t stream) {
     const size_t smem = masked ? 0 : (size_t)per * 16;
     a.cluster = cluster;
     auto kernel = masked ? loss_masked_kernel<T, kDense> : loss_kernel<T, kDense>;
-    // (48 KB go without asking, the kernel's own few included)
-    if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (48 KB go without asking, the kernel's own few included; the limit is the
+    // kernel's, not the call's: every call asks for the same, so that calls of
+    // several threads do not take it from each other)
+    if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostScores);
     if (e == cudaSuccess && cluster == 16)
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) break;

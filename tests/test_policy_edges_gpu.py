@@ -1,5 +1,8 @@
 """The policy loss and sampling at the edges of their inputs, against the plain
 restatements in 64 bits (tests/policy_ref.py)."""
+import ctypes as C
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -111,3 +114,31 @@ def test_a_wait_that_runs_out_leaves_nan(cuda):
     assert gz.selftest_cluster_wait_timeout(0, 20000) == gz.ERR_TIMEOUT
     assert gz.selftest_cluster_wait_timeout(0, 0) == gz.ERR_INVALID_ARG
     check_loss(rows_of(3, 60000, 1), label=torch.arange(3, dtype=torch.int32))
+
+
+def test_loss_from_several_threads(cuda):
+    """Calls at once, whose rows want different amounts of shared memory, do not refuse each other."""
+    calls, refused = [], []
+    for a in (24000, 50000, 30000, 44000):
+        x = torch.zeros(1, a, dtype=torch.bfloat16, device="cuda").expand(200, a)
+        label, loss = torch.zeros(200, dtype=torch.int32, device="cuda"), torch.empty(200, device="cuda")
+        rows = gz.PolicyRows(x.data_ptr(), None, 0, 0, 200, a, gz.BF16)
+        calls.append((x, label, loss, rows, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def work(x, label, loss, rows, stream):
+        for _ in range(4000):
+            status = gz._lib.gz_policy_loss(C.byref(rows), None, 0, label.data_ptr(), None, 1.0, loss.data_ptr(), None, 0,
+                                            stream.cuda_stream)
+            if status != gz.OK:
+                refused.append(status)
+
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused
+    for x, _, loss, _, _ in calls:
+        assert (loss - np.log(x.shape[1])).abs().max() <= 1e-4
