@@ -195,8 +195,9 @@ struct Filters {
   bool greedy;  // the best action alone
 
   __device__ Filters(const gz_sample_config& c, int64_t row) {
-    temperature = fminf(c.d_temperature ? c.d_temperature[row] : c.temperature, FLT_MAX);
-    if (temperature > 0.f) temperature = fmaxf(temperature, 1e-30f);  // its reciprocal stays finite
+    // (of a NaN the end that keeps the fewest actions is taken: 0, 0 and 1)
+    temperature = c.d_temperature ? c.d_temperature[row] : c.temperature;
+    if (temperature > 0.f) temperature = fminf(fmaxf(temperature, 1e-30f), FLT_MAX);  // its reciprocal stays finite
     top_p = c.d_top_p ? c.d_top_p[row] : c.top_p;
     min_p = fminf(c.d_min_p ? c.d_min_p[row] : c.min_p, 1.f);
     top_k = c.d_top_k ? c.d_top_k[row] : c.top_k;

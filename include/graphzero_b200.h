@@ -413,7 +413,8 @@ typedef struct {
 } gz_policy_rows;
 /* How actions are drawn.  Each setting is one value for all rows, or a device
  * array [rows] where its pointer is not NULL (values out of range are then
- * taken as the nearest end of the range).
+ * taken as the nearest end of the range, a NaN as the end that keeps the fewest
+ * actions: temperature 0, top_p 0, min_p 1).
  *   temperature  >= 0; 0 picks the best action
  *   top_k        only the k best actions; 0: all
  *   top_p        of those, the best ones until their share reaches top_p; 1: all

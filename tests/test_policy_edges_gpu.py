@@ -142,3 +142,20 @@ def test_loss_from_several_threads(cuda):
     assert not refused
     for x, _, loss, _, _ in calls:
         assert (loss - np.log(x.shape[1])).abs().max() <= 1e-4
+
+
+@pytest.mark.parametrize("a,share", [(7, None), (500, None), (4672, 0.01), (20000, None), (20000, 0.5)])
+def test_sample_settings_of_nan_keep_the_best(cuda, a, share):
+    """A NaN in a row's setting is taken as the value that keeps the fewest actions."""
+    n = 6
+    x, noise = rows_of(n, a, 1).cuda(), ref.gumbel((n, a), 2).cuda()
+    mask = None if share is None else (torch.rand(n, a, device="cuda") < share).to(torch.uint8)
+    best = gz.policy_sample(x, noise, mask=mask, temperature=0.0)
+    plain = gz.policy_sample(x, noise, mask=mask)
+    for kw, rest in (("temperature", 1.0), ("top_p", 1.0), ("min_p", 0.0)):
+        v = torch.full((n,), float("nan"), device="cuda")
+        v[::2] = rest
+        got = gz.policy_sample(x, noise, mask=mask, **{kw: v})
+        for k in (0, 1):
+            assert torch.equal(got[k][1::2], best[k][1::2]), kw
+            assert torch.equal(got[k][::2], plain[k][::2]), kw
