@@ -130,7 +130,9 @@ __device__ __forceinline__ bool grads_aligned(const void* g, int dtype) {
 }
 
 // Sum of squares: eight products added in pairs in 32 bits, everything above
-// them in 64.  One block's last arrival adds the chunks' sums, in their order.
+// them in 64.  Where 32 bits do not hold the products (gradients beyond 2^64
+// overflow; below a sum of 2^-100 lost bits could count) those are taken in 64
+// too.  One block's last arrival adds the chunks' sums, in their order.
 __global__ void __launch_bounds__(kThreads) norm_kernel(StepArgs a, const __grid_constant__ Grads grads) {
   __shared__ double sums[kThreads / 32];
   __shared__ bool last;
@@ -148,9 +150,16 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(StepArgs a, const __grid
       if (at >= n) break;
       float x[kPerLane];
       load_grads(x, g, dtype, at, lane, n, aligned && at + kBlock <= n);
+      float y[kPerLane];
 #pragma unroll
-      for (int k = 0; k < kPerLane; ++k) x[k] *= x[k];
-      sum += (double)(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
+      for (int k = 0; k < kPerLane; ++k) y[k] = x[k] * x[k];
+      const float s = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+      if (s >= 0x1p-100f && s < INFINITY) {
+        sum += (double)s;
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPerLane; ++k) sum += (double)x[k] * x[k];
+      }
     }
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
   if (lane == 0) sums[threadIdx.x / 32] = sum;

@@ -227,3 +227,18 @@ def test_steps_of_a_plan_without_gradients_count(cuda):
         with pytest.raises((ValueError, gz.GZError)):
             opt.steps = bad
     assert opt.steps == 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1e-22, 1e-15, 1e15, 1e19, 1e22, 1e30, 1e34])
+def test_norm_over_the_range_of_the_gradients(cuda, size, dtype):
+    """Squares that 32 bits do not hold count too, in whole blocks and ragged ends.
+    The sum is taken in 64 bits and rounded once; a norm below 2^-126 to a
+    multiple of 2^-149."""
+    shapes = [(4, 256), (301,)]
+    gs = [(g / 1e-3 * size).to(dtype) for g in gradients(shapes, 3)]
+    params = make(shapes)
+    norm = gz.AdamW(params, max_norm=1.0).step(gs)
+    want = float(torch.sqrt(sum((g.double() ** 2).sum() for g in gs)))
+    assert abs(float(norm) - want) <= 2 * U * want + 2.0**-149
+    assert all(p.isfinite().all() for p in params)
