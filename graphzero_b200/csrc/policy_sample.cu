@@ -511,6 +511,7 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
   const float* noise = r.noise ? r.noise + r.head : nullptr;
   const bool aligned = ((uintptr_t)noise & 15) == 0;
   const float least = last ? key_score(last) : -FLT_MAX, per = 1.f / f.temperature;
+  const float above = least < FLT_MAX ? least : INFINITY;  // kept whatever its index is; +inf counts as FLT_MAX
   const int last_index = last ? key_index(last) : GZ_POLICY_MAX_ACTIONS;
   float most = -INFINITY, z = 0.f;
   uint64_t weight = 0;  // the same in whole numbers, under a mask: whatever the mask's alignment to the scores
@@ -528,7 +529,7 @@ __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const bool kept = x[k] > least || (x[k] == least && r.head + v * V + k <= last_index);
+      const bool kept = x[k] > above || (x[k] >= least && r.head + v * V + k <= last_index);
       x[k] = kept ? fminf(x[k], FLT_MAX) : -INFINITY;
     }
   };

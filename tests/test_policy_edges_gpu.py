@@ -9,7 +9,7 @@ import torch
 
 import graphzero_b200 as gz
 import policy_ref as ref
-from test_policy_gpu import DTYPES, U, check_loss, rows_of
+from test_policy_gpu import DTYPES, U, check_loss, check_sample, legal, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +159,21 @@ def test_sample_settings_of_nan_keep_the_best(cuda, a, share):
         for k in (0, 1):
             assert torch.equal(got[k][1::2], best[k][1::2]), kw
             assert torch.equal(got[k][::2], plain[k][::2]), kw
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("a,share", [(300, None), (2000, None), (4672, 0.9), (9001, None), (40000, None), (40000, 0.9)])
+def test_sample_scores_of_infinity_tie(cuda, a, share, dtype):
+    """Scores of +inf are the largest float: of many such, and of the largest
+    finite score beside them, the filters keep the lowest indices."""
+    n = 6
+    g = torch.Generator().manual_seed(a)
+    x, noise = rows_of(n, a, a, dtype), ref.gumbel((n, a), a + 3)
+    for i, many in enumerate((2, 9, 44, 44, a // 2, a)):
+        x[i, torch.randperm(a, generator=g)[:many]] = float("inf")
+    x[3, torch.randperm(a, generator=g)[:20]] = torch.finfo(dtype).max
+    x[3, :a // 8] = float("nan")
+    mask = None if share is None else legal(n, a, share, 5)
+    for kw in (dict(top_p=0.5), dict(top_k=a - 1, top_p=0.95, temperature=0.001), dict(top_k=a - 1, top_p=0.9, temperature=0.3),
+               dict(top_k=30), dict(top_k=a // 3), dict(top_p=0.95, min_p=0.5), dict()):
+        check_sample(x, noise, mask, **kw)
