@@ -763,7 +763,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
     unpack<T>(r.vector(where), x);
 #pragma unroll
     for (int k = V - 1; k >= 0; --k)
-      if (fminf(x[k], FLT_MAX) == most) best = rank_key(most, r.head + where * V + k);
+      if (x[k] >= most) best = rank_key(most, r.head + where * V + k);  // (+inf counts as FLT_MAX, a NaN is none)
   }
   z = sum.x + sum.y;
   if (tid < r.ends) {

@@ -177,3 +177,20 @@ def test_sample_scores_of_infinity_tie(cuda, a, share, dtype):
     for kw in (dict(top_p=0.5), dict(top_k=a - 1, top_p=0.95, temperature=0.001), dict(top_k=a - 1, top_p=0.9, temperature=0.3),
                dict(top_k=30), dict(top_k=a // 3), dict(top_p=0.95, min_p=0.5), dict()):
         check_sample(x, noise, mask, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("a,share", [(7, None), (60, 0.9), (300, None), (2000, None), (4672, 0.9), (9001, None), (40001, None),
+                                     (40001, 0.9)])
+def test_sample_nan_beside_infinity_is_never_picked(cuda, a, share, dtype):
+    """Rows of NaN but for a few scores of +inf, of the largest float, or ordinary ones."""
+    n = 12
+    g = torch.Generator().manual_seed(a)
+    x, noise = torch.full((n, a), float("nan"), dtype=dtype), ref.gumbel((n, a), a + 4)
+    for i in range(n):
+        at = torch.randperm(a, generator=g)[:1 + i // 3]
+        x[i, at] = (float("inf"), torch.finfo(dtype).max, 1.5)[i % 3]
+    mask = None if share is None else legal(n, a, share, 6)
+    for kw in (dict(temperature=0.0), dict(top_k=1), dict(top_p=0.0), dict(top_k=2), dict(top_p=0.4), dict(min_p=1.0), dict()):
+        check_sample(x, noise, mask, **kw)
+    check_sample(x, None, mask)
