@@ -454,7 +454,9 @@ gz_status gz_policy_sample(const gz_policy_rows* rows, const gz_sample_config* c
  * the loss too) is NaN in that row and in the rows that it would have done
  * after it.  d_loss [rows] fp32; d_grad [rows][actions] of the logits'
  * dtype, NULL for the loss alone, and it overlaps no input.  fp32 inside,
- * in an order that depends on the row's length and alignment only. */
+ * in an order that depends on the row's length, alignment and mask and on the
+ * number of rows (few long rows are split over more blocks), not on what other
+ * rows hold: the same call gives the same bits. */
 gz_status gz_policy_loss(const gz_policy_rows* rows, const float* d_target, int64_t target_stride,
                          const int32_t* d_label, const float* d_weight, float grad_scale, float* d_loss, void* d_grad,
                          int64_t grad_stride, void* stream);

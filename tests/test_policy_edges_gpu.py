@@ -108,6 +108,22 @@ def test_loss_of_scores_of_any_magnitude(cuda, n, a, share, dtype):
         assert (np.abs(grad.float().cpu().numpy() - wgrad) <= bound).all()
 
 
+@pytest.mark.parametrize("n,a,share", [(40, 300, None), (40, 4672, 0.01), (40, 9000, 0.5), (200, 9000, None), (5, 131072, None),
+                                       (5, 131072, 0.5)])
+def test_loss_of_a_row_does_not_depend_on_other_rows(cuda, n, a, share):
+    """In calls of as many rows: the same bits whatever the others hold, and again for the same call."""
+    mask = None if share is None else legal(n, a, share, 1).cuda()
+    x, label = rows_of(n, a, 2, torch.bfloat16).cuda(), torch.arange(n, dtype=torch.int32, device="cuda")
+    loss, grad = gz.policy_loss(x, label=label, mask=mask)
+    again = gz.policy_loss(x, label=label, mask=mask)
+    assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+    for i in (0, n // 2, n - 1):
+        y = rows_of(n, a, 3 + i, torch.bfloat16, spread=9.0).cuda()
+        y[i] = x[i]
+        got = gz.policy_loss(y, label=label, mask=mask)
+        assert torch.equal(got[0][i], loss[i]) and torch.equal(got[1][i], grad[i])
+
+
 def test_a_wait_that_runs_out_leaves_nan(cuda):
     """Blocks that share a row wait for sums that nothing sends: the waits give
     up after their limit, the results are NaN, and the next call is right."""
