@@ -20,7 +20,9 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "gz_internal.h"
@@ -529,6 +531,30 @@ struct Device {  // the plan's device for the scope
   }
 };
 
+// Whether two of the buffers that a step writes overlap: blocks of threads would
+// race for them.
+bool any_overlap(const std::vector<Tensor>& tensors, int state_bits) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  auto add = [&](const void* p, uint64_t bytes) {
+    if (p && bytes) spans.push_back({(uintptr_t)p, (uintptr_t)p + bytes});
+  };
+  for (const Tensor& t : tensors) {
+    const uint64_t n = (uint64_t)t.n, blocks = (n + kBlock - 1) / kBlock, state = state_bits == 8 ? blocks * kBlock : 4 * n;
+    add(t.param, 4 * n);
+    add(t.copy, 2 * n);
+    add(t.m, state);
+    add(t.v, state);
+    if (state_bits == 8) {
+      add(t.m_scale, 4 * blocks);
+      add(t.v_scale, 4 * blocks);
+    }
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t k = 1; k < spans.size(); ++k)
+    if (spans[k].first < spans[k - 1].second) return true;
+  return false;
+}
+
 gz_status create(const gz_adamw_tensor* tensors, int count, int state_bits, int device, gz_adamw* a) {
   const char* who = "gz_adamw_create";
   std::vector<Tensor> table((size_t)count);
@@ -549,6 +575,7 @@ gz_status create(const gz_adamw_tensor* tensors, int count, int state_bits, int 
                 t.copy_dtype};
     first += (uint64_t)(t.n + kBlock - 1) / kBlock * kBlock;
   }
+  if (any_overlap(table, state_bits)) return bad(who, "weights, copies or states overlap");
   a->device = device;
   a->state_bits = state_bits;
   a->count = count;

@@ -498,7 +498,8 @@ typedef struct {
 } gz_adamw_config;
 typedef struct gz_adamw gz_adamw;
 /* A plan over `count` tensors of `device` (host array; the buffers stay the
- * caller's).  state_bits 8 or 32.  Allocates and synchronises. */
+ * caller's; those that steps write must not overlap, a weight that two layers
+ * share is given once).  state_bits 8 or 32.  Allocates and synchronises. */
 gz_status gz_adamw_create(const gz_adamw_tensor* tensors, int count, int state_bits, int device, gz_adamw** out);
 gz_status gz_adamw_destroy(gz_adamw* a);
 /* One step.  d_grads: host array of `count` device pointers [n], NULL for a
