@@ -880,12 +880,14 @@ class AdamW:
     A step can be captured in a CUDA graph; every replay is then a step with the
     next t, on the gradients at the captured addresses, with the capture's lr
     and other settings.  `steps` counts replays too: it is read from the device
-    once a step has been captured, and reading it waits for the device then."""
+    once a step has been captured, and reading it waits for the device then.
+    Keep the AdamW and its tensors, and do not close it, while such a graph is
+    in use."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, copies=None,
                  lr_scale=1.0, max_norm=0.0, seed=0):
         torch = _need_torch()
-        self._plan = _vp()
+        self._plan, self._counted = _vp(), False  # whether t is the device's to count: after a capture
         self._params = tuple(params)
         count = len(self.params)
         each = lambda x: list(x) if isinstance(x, (list, tuple)) else [x] * count  # noqa: E731
@@ -904,7 +906,7 @@ class AdamW:
                                   or c.device != self.device or not c.is_contiguous()):
                 raise ValueError("copies must be contiguous float16 or bfloat16 tensors of their weights' shapes")
         self.lr, self.betas, self.eps, self.max_norm, self.seed = lr, tuple(betas), eps, max_norm, seed
-        self._steps, self._counted = 0, False  # whether t is the device's to count
+        self._steps = 0
         self.offsets, total = [], 0
         for p in self.params:
             self.offsets.append(total)
@@ -960,7 +962,8 @@ class AdamW:
 
     def __del__(self):
         try:
-            self.close()
+            if not self._counted:  # a captured step's graph may outlive this object: its plan is kept
+                self.close()
         except Exception:  # noqa: BLE001
             pass
 

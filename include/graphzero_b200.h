@@ -512,7 +512,7 @@ gz_status gz_adamw_destroy(gz_adamw* a);
  * the gradients among them.  With cfg->step 0 every replay is a step of its own:
  * t, and with it the bias corrections and the rounding numbers, goes on from
  * wherever calls and replays before it have left it.  (With another cfg->step
- * every replay repeats that t.) */
+ * every replay repeats that t.)  The plan must outlive its graphs. */
 gz_status gz_adamw_step(gz_adamw* a, const void* const* d_grads, const int32_t* grad_dtypes,
                         const gz_adamw_config* cfg, float* d_norm, void* stream);
 /* The number t of the plan's last step (0 before the first), and setting it (a

@@ -1,5 +1,7 @@
 """AdamW: its states' types, gradients and norms that are not finite, captures
 replayed, and tensors that have moved."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -242,3 +244,29 @@ def test_norm_over_the_range_of_the_gradients(cuda, size, dtype):
     want = float(torch.sqrt(sum((g.double() ** 2).sum() for g in gs)))
     assert abs(float(norm) - want) <= 2 * U * want + 2.0**-149
     assert all(p.isfinite().all() for p in params)
+
+
+def test_a_captured_plan_outlives_its_object(cuda, monkeypatch):
+    """A graph's replays read the plan: collecting the AdamW must not free it (close() does)."""
+    freed = []
+    destroy = gz._lib.gz_adamw_destroy
+    monkeypatch.setattr(gz._lib, "gz_adamw_destroy", lambda plan: freed.append(plan.value) or destroy(plan))
+    for capture in (False, True):
+        params, gs = make([(300,)]), gradients([(300,)], 1)
+        opt = gz.AdamW(params)
+        if capture:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step(gs)
+            del graph
+        else:
+            opt.step(gs)
+        plan = opt._plan.value
+        del opt
+        gc.collect()
+        assert (plan in freed) == (not capture)
+    destroy(plan)  # (nothing uses it any more here)
+    opt = gz.AdamW(params)
+    plan = opt._plan.value
+    opt.close()
+    assert freed[-1] == plan
