@@ -8,8 +8,7 @@
 // and the rest is done there, by one warp where the list is short:
 //  - Masked rows of up to 5120 actions (legal moves): a warp lists the visible
 //    ones, sixteen mask bytes at a time, and reads scores and noise of these
-//    alone.  4096 rows of 4672 with top_p and min_p: 13 us, 4.4 TB/s of scores
-//    and mask.
+//    alone.  4096 rows of 4672 with top_p and min_p: 13 us, 1.5 TB/s of mask.
 //  - Other rows: a block reads the row once for its best score, its vectors'
 //    maxima and, where top_p needs it, its sum of exponentials.  A bound below
 //    which (nearly always) nothing is kept gives the list (draw_long).  256 rows
@@ -46,7 +45,7 @@ constexpr int kList = 2048;          // keys a block's list holds
 constexpr int kMaskedList = 1024, kMaskedThreads = 128;  // the same for blocks of four masked rows, and their threads
 constexpr int kSampleThreads = 512;  // most threads of a block
 constexpr int kReachBit = 16;       // lowest bit of a score that the search for a list's bound looks at
-constexpr int kMaximaVecs = 24576;  // vectors of a row whose maxima are kept (96 KB: two blocks fit an SM)
+constexpr int kMaximaVecs = 24576;  // vectors of a row whose maxima are kept (96 KB; up to 22700 two blocks fit an SM)
 constexpr int64_t kRowsPerLaunch = 1 << 28;
 
 // e = exp(d), 0 .. 1, in units of 2^-44, cut off: 2^18 actions sum below 2^63.
@@ -502,7 +501,9 @@ template <int kSize> struct Shared {
 // bits (under a mask in whole numbers).  Noisy scores are compared as they are
 // defined, but with a temperature the division is done only for vectors whose
 // upper bound, from a product with its reciprocal, could still win.  256
-// unfiltered rows of 131072: 63 us, 1.6 TB/s, bound by instructions.
+// unfiltered rows of 131072 bf16 scores, draw_long's pass included: 60 us at
+// temperature 1, 76 us at 0.8 (3.3 and 2.7 TB/s of scores and noise), bound by
+// instructions.
 template <typename T, bool kMask>
 __device__ void draw_from_all(const SampleArgs& a, int64_t row, const Team<false>& team, const Row<T, kMask>& r, const Filters& f, float top,
                               uint64_t last) {
@@ -790,7 +791,7 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
     if (row_weighs) {
       if (__syncthreads_and(z_fine)) {
         z *= z_base > -INFINITY ? sm100::ex2_approx((z_base - top) * per_score) : 0.f;
-      } else {  // beyond what a sum relative to some score holds, or under a mask
+      } else {  // beyond what a sum relative to some score holds
         z = 0.f;
         each(r, tid, n, [&](int, float x) { z += expf(f.depth(x, top)); });
       }
@@ -798,6 +799,11 @@ __device__ __forceinline__ void draw_long(const SampleArgs& a, int64_t row, Shar
     }
     // Bounds for the list.  For top_k the largest number that top_k threads' best
     // scores reach; one warp searches for it, over the scores' upper 16 bits.
+    // Not so where top_k is above the number of threads, nor where the leading
+    // bits that those scores' keys share are all 0 (scores on both sides of 0, or
+    // of -2 where none is positive): such rows have no list and take the
+    // histogram (256 rows of 131072 with top_k 50: 26 us with the list, 229 us
+    // with scores 4 lower that do without).
     // For top_p the scores of a weight of 1/256, then 1/2048 of what top_p leaves
     // out; no more than 256 / (1 - top_p) actions reach the first, and what lies
     // below it is often little.  Rows of up to kList actions are flatter at
