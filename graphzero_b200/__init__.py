@@ -13,6 +13,7 @@ broadcast_weights) and its factory create_neural_net(type, game)
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 import struct
 from pathlib import Path
@@ -952,6 +953,7 @@ class AdamW:
 
     @steps.setter
     def steps(self, n):
+        n = operator.index(n)
         _check(_lib.gz_adamw_set_steps(self._plan, n))
         self._steps = n
 

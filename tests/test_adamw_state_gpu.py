@@ -270,3 +270,13 @@ def test_a_captured_plan_outlives_its_object(cuda, monkeypatch):
     plan = opt._plan.value
     opt.close()
     assert freed[-1] == plan
+
+
+def test_steps_take_any_whole_number(cuda):
+    opt = gz.AdamW(make([(9,)]))
+    for n in (3, np.int64(4), torch.tensor(5)):
+        opt.steps = n
+        assert opt.steps == int(n) and type(opt.steps) is int
+    with pytest.raises(TypeError):
+        opt.steps = 2.5
+    assert opt.steps == 5
